@@ -551,7 +551,7 @@ def _exact_codes(x):
     codes' values and the scale bytes."""
     x = x.double()
     m, e = torch.frexp(x.abs().amax(-1))  # max |x| = m 2^e, 0.5 <= m < 1; 448 = 0.875 * 2^9
-    e = torch.where(m > 0.875, e - 8, e - 9).clamp_min(-126)
+    e = torch.where(m > 0.875, e - 8, torch.where(m > 0, e - 9, -126)).clamp_min(-126)
     y = x / _two_to(e)[..., None]
     quantum = _two_to((torch.frexp(y)[1] - 1).clamp_min(-6) - 3)
     return torch.round(y / quantum) * quantum, e + 127
