@@ -60,6 +60,20 @@ class AttnDesc(ctypes.Structure):
                 ("tile_pages", _I)]
 
 
+class Kv8Cache(ctypes.Structure):
+    """The pools of an 8-bit paged K/V cache (cbis_kv8_cache)."""
+    _fields_ = [("n_kv_heads", _I), ("head_dim", _I), ("page_size", _I), ("num_pages", _I),
+                ("k_pool", _P), ("v_pool", _P)]
+
+
+class Kv8AttnDesc(ctypes.Structure):
+    _fields_ = [("cache", Kv8Cache), ("n_rows", _I), ("rows", _P), ("n_heads", _I),
+                ("q_dtype", _I), ("q", _P), ("ldq", _I64),
+                ("block_table", _P), ("bt_stride", _I64), ("row_bt", _P), ("row_pos", _P),
+                ("out_dtype", _I), ("out", _P), ("ldo", _I64),
+                ("max_kv_len", _I), ("split_tokens", _I), ("workspace", _P), ("workspace_bytes", _SZ)]
+
+
 class EvictionParams(ctypes.Structure):
     """include/tiered_kv_manager.hpp:40-48."""
     _fields_ = [("alpha_staleness", ctypes.c_double), ("beta_restore_cost", ctypes.c_double),
@@ -107,6 +121,13 @@ KERNEL_SYMBOLS = {
     "cbis_paged_prefill_attention": (_I, [ctypes.POINTER(AttnDesc), _I, _P, _P]),
     "cbis_paged_chunk_attention": (_I, [ctypes.POINTER(AttnDesc), _I, _P, _P]),
     "cbis_paged_attention_mixed": (_I, [ctypes.POINTER(AttnDesc), _I, _P, _P]),
+    "cbis_kv8_page_bytes": (_SZ, [_I, _I, _I]),
+    "cbis_kv8_scatter": (_I, [ctypes.POINTER(Kv8Cache), _I, _I, _P, _I64, _P, _I64, _P, _P, _P]),
+    "cbis_kv8_gather": (_I, [ctypes.POINTER(Kv8Cache), _I, _I, _P, _I64, _P, _I64, _P, _P, _P]),
+    "cbis_kv8_attention_workspace_size": (_SZ, [ctypes.POINTER(Kv8AttnDesc)]),
+    "cbis_kv8_attention": (_I, [ctypes.POINTER(Kv8AttnDesc), _P]),
+    "cbis_kv8_chunk_attention_workspace_size": (_SZ, [ctypes.POINTER(Kv8AttnDesc), _I]),
+    "cbis_kv8_chunk_attention": (_I, [ctypes.POINTER(Kv8AttnDesc), _I, _P, _P]),
     "cbis_embed": (_I, [_I, _I, _P, _P, _I, _P, _P, _I, _I, _P, _P]),
     "cbis_embed_from": (_I, [_I, _I, _P, _P, _P, _P, _I, _P, _P, _I, _I, _P, _P, _P, _SZ, _P]),
     "cbis_layernorm": (_I, [_I, _I, _P, _I64, _P, _P, _F, _I, _P, _I64, _P]),

@@ -1,0 +1,1159 @@
+// The 8-bit paged K/V cache: rows quantised into their page slots, slots read
+// back, and the attention of single rows and of chunks of rows over the pages.
+// The reference keeps its cache in fp32 only (kernels/attention.cu:7-127); a
+// decode step of long sequences is bound by the cache's bytes, which this
+// format cuts to (head_dim + 1) / (2 head_dim) of bf16's.
+//
+// Number format.  The K (or V) slice of one token and head, x[0 .. d), is held
+// as OCP e4m3 codes c and one exponent byte b:
+//   e = the least integer >= -126 with max |x| <= 448 * 2^e,  b = e + 127,
+//   c_i = RNE_e4m3(x_i * 2^-e),  value_i = c_i * 2^e.
+// The scale is a power of two, so x * 2^-e is exact and each element is rounded
+// once, to nearest even: at most 2^-4 of its value (half a step of 3 mantissa
+// bits), or 2^-10 * 2^e below the normal codes.  A slice with a NaN or an
+// infinity gets b = 255 and zero codes, and reads as NaN throughout: a stored
+// code is never e4m3's NaN, so a bad slice cannot reach other heads or tokens
+// that share a matrix instruction with it.
+//
+// Page layout.  A page is page_size / 16 tiles of 16 tokens; a K tile is codes
+// [kv_heads][16][d] then bytes [kv_heads][16], a V tile codes [kv_heads][d][16]
+// then bytes [kv_heads][16].  Both are laid out for v_mfma_f32_16x16x32: the
+// scores' A operand is 16 tokens by d (lane: one token, consecutive dims), the
+// output's A operand 16 dims by tokens (lane: one dim, consecutive tokens), so
+// each lane's operand bytes are consecutive in memory and go from the load
+// through one conversion straight into the instruction.
+#include <algorithm>
+#include <cmath>
+
+#include "common.hpp"
+
+namespace cbis {
+namespace {
+
+typedef __bf16 bf16v8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16v2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16v8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kTile = 16;          // tokens of a cache tile
+constexpr int kBlk = 64;           // tokens a wave takes at a time: four tiles
+constexpr int kBadByte = 255;      // scale byte of a slice with a non-finite value
+constexpr int kDecodeWaves = 8;
+constexpr int kChunkWaves = 4;
+constexpr float kLowest = -3.3e38f;  // a running maximum before any score
+
+// ---------------------------------------------------------------------------
+// Addressing.
+// ---------------------------------------------------------------------------
+struct Pages {
+  uint8_t *k, *v;
+  int num_pages, page_size;
+  int tshift;  // log2 of the tiles of a page
+  int kv_heads, head_dim;
+  int64_t tile_bytes;
+};
+
+// Byte offset of tile t of the sequence with block-table row bt.  Page ids are
+// clamped to the pool; the offset passes 32 bits in large pools.
+__device__ inline int64_t tile_offset(const Pages& c, const int* __restrict__ bt, int t) {
+  const unsigned page = min((unsigned)bt[t >> c.tshift], (unsigned)(c.num_pages - 1));
+  return (((int64_t)page << c.tshift) + (t & ((1 << c.tshift) - 1))) * c.tile_bytes;
+}
+
+__device__ inline float pow2_of_byte(unsigned b) { return __uint_as_float(b << 23); }
+
+// ---------------------------------------------------------------------------
+// Write: one group of lanes per slice (row, K | V, head), 16 bytes of input
+// per lane.  HBM-bound; see the launch for its figures.
+// ---------------------------------------------------------------------------
+struct RowsArgs {
+  Pages c;
+  int n_rows;
+  const void *k, *v;
+  int64_t ldk, ldv;
+  const int *page, *offset;
+};
+
+template <typename T>
+struct RowElems {
+  static constexpr int kPerLane = 16 / sizeof(T);
+};
+
+template <typename T, bool kVec>
+__device__ inline void load_elems(const T* p, float* x) {
+  constexpr int N = RowElems<T>::kPerLane;
+  if constexpr (kVec) {
+    const u32x4_t w = __builtin_nontemporal_load((const u32x4_t*)p);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = bf16lo(w[i]);
+        x[2 * i + 1] = bf16hi(w[i]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (sizeof(T) == 4) x[i] = ((const float*)p)[i];
+      else x[i] = bf16_to_f32(((const uint16_t*)p)[i]);
+    }
+  }
+}
+
+template <typename T, int HD, bool kVec>
+__global__ __launch_bounds__(256) void kv8_scatter_kernel(const RowsArgs a) {
+  constexpr int N = RowElems<T>::kPerLane, L = HD / N;
+  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int sub = (int)(gid % L);
+  const int64_t slice = gid / L;
+  const int H = a.c.kv_heads;
+  const int64_t row = slice / (2 * H);
+  if (row >= a.n_rows) return;  // whole groups only: a group is one slice
+  const int rest = (int)(slice % (2 * H));
+  const bool is_v = rest >= H;
+  const int head = is_v ? rest - H : rest;
+  const int page = a.page[row], off = a.offset[row];
+  if ((unsigned)page >= (unsigned)a.c.num_pages || (unsigned)off >= (unsigned)a.c.page_size) return;
+  const T* src = is_v ? (const T*)a.v + row * a.ldv : (const T*)a.k + row * a.ldk;
+  float x[N];
+  load_elems<T, kVec>(src + head * HD + sub * N, x);
+  unsigned top = 0;  // max |x| by its bits: NaN above infinity above every finite value
+#pragma unroll
+  for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int m = 1; m < L; m *= 2) top = max(top, (unsigned)__shfl_xor((int)top, m, 64));
+  const bool bad = top >= 0x7F800000u;
+  // max |x| = 1.m * 2^(E - 127) <= 448 * 2^e = 1.75 * 2^(8 + e): e + 127 = E - 8,
+  // one more where 1.m > 1.75.
+  const int byte = bad ? kBadByte : max(1, (int)(top >> 23) - 8 + ((top & 0x7FFFFFu) > 0x600000u));
+  const float inv = bad ? 0.f : pow2_of_byte((unsigned)(254 - byte));
+  uint32_t w[N / 4];
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    int d = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inv, x[4 * i + 1] * inv, 0, false);
+    d = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inv, x[4 * i + 3] * inv, d, true);
+    w[i] = bad ? 0u : (uint32_t)d;
+  }
+  const int slot = off & (kTile - 1);
+  uint8_t* tile = (is_v ? a.c.v : a.c.k) + (((int64_t)page << a.c.tshift) + (off >> 4)) * a.c.tile_bytes;
+  if (is_v) {
+    uint8_t* dst = tile + ((int64_t)head * HD + sub * N) * kTile + slot;
+#pragma unroll
+    for (int i = 0; i < N; ++i) dst[i * kTile] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
+  } else {
+    uint8_t* dst = tile + ((int64_t)head * kTile + slot) * HD + sub * N;
+    if constexpr (N == 4) *(uint32_t*)dst = w[0];
+    else *(uint2*)dst = make_uint2(w[0], w[1]);
+  }
+  if (sub == 0) tile[(int64_t)H * HD * kTile + head * kTile + slot] = (uint8_t)byte;
+}
+
+// ---------------------------------------------------------------------------
+// Read back: the same groups the other way.
+// ---------------------------------------------------------------------------
+template <typename T, int HD, bool kVec>
+__global__ __launch_bounds__(256) void kv8_gather_kernel(const RowsArgs a) {
+  constexpr int N = RowElems<T>::kPerLane, L = HD / N;
+  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int sub = (int)(gid % L);
+  const int64_t slice = gid / L;
+  const int H = a.c.kv_heads;
+  const int64_t row = slice / (2 * H);
+  if (row >= a.n_rows) return;
+  const int rest = (int)(slice % (2 * H));
+  const bool is_v = rest >= H;
+  const int head = is_v ? rest - H : rest;
+  const int page = a.page[row], off = a.offset[row];
+  if ((unsigned)page >= (unsigned)a.c.num_pages || (unsigned)off >= (unsigned)a.c.page_size) return;
+  const int slot = off & (kTile - 1);
+  const uint8_t* tile = (is_v ? a.c.v : a.c.k) + (((int64_t)page << a.c.tshift) + (off >> 4)) * a.c.tile_bytes;
+  uint32_t w[N / 4];
+  if (is_v) {
+    const uint8_t* src = tile + ((int64_t)head * HD + sub * N) * kTile + slot;
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      w[i] = src[(4 * i) * kTile] | src[(4 * i + 1) * kTile] << 8 | src[(4 * i + 2) * kTile] << 16 |
+             (uint32_t)src[(4 * i + 3) * kTile] << 24;
+  } else {
+    const uint8_t* src = tile + ((int64_t)head * kTile + slot) * HD + sub * N;
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) w[i] = ((const uint32_t*)src)[i];
+  }
+  const float scale = pow2_of_byte(tile[(int64_t)H * HD * kTile + head * kTile + slot]);
+  float x[N];
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
+    const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+    x[4 * i] = lo[0] * scale;
+    x[4 * i + 1] = lo[1] * scale;
+    x[4 * i + 2] = hi[0] * scale;
+    x[4 * i + 3] = hi[1] * scale;
+  }
+  T* dst = (T*)(is_v ? a.v : a.k) + row * (is_v ? a.ldv : a.ldk) + head * HD + sub * N;
+  if constexpr (kVec) {
+    u32x4_t o;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = __float_as_uint(x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    }
+    __builtin_nontemporal_store(o, (u32x4_t*)dst);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (sizeof(T) == 4) ((float*)dst)[i] = x[i];
+      else ((uint16_t*)dst)[i] = f32_to_bf16(x[i]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention.
+//
+// Both kernels compute S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32
+// over blocks of 64 tokens (four tiles).  Row m of the scores' p-th product is
+// token 4 p + m % 4 of tile m / 4, so a lane's accumulators over p = 0 .. 3 are
+// the 16 tokens of tile lane / 16 for column lane % 16 -- which is the k order
+// in which a lane's 16 consecutive V bytes of a dim enter the second product:
+// probabilities never cross lanes.
+//
+// Numbers.  e4m3 codes are exact in bf16 (scores) and f16 (output).  q enters
+// as QP bf16 parts: one for bf16 q; two (16 bits) for fp32 q and a bf16 result;
+// three (all 24 bits) for fp32 q and an fp32 result.  The probabilities enter
+// as PP f16 parts: one (11 bits) for a bf16 result, whose own rounding is 8
+// bits; two (22 bits) for fp32.  f16's range is kept by two references per
+// column, both raised only when a block needs it: m, with p = 2^(s - m + 8) <=
+// 2^15 (s in log2 units), and E, a bound on the V scales' bytes.  Scores, sums
+// and outputs are fp32.
+// ---------------------------------------------------------------------------
+struct AttnArgs {
+  Pages c;
+  int n_rows, n_heads, group;
+  const int* rows;
+  const void* q;
+  int64_t ldq;
+  int q_bf16, q_vec;
+  const int* bt;
+  int64_t bt_stride;
+  const int *row_bt, *row_pos;
+  void* out;
+  int64_t ldo;
+  int out_bf16, out_vec;
+  int max_tok;       // tokens a block-table row covers
+  float qscale;      // log2(e) / sqrt(head_dim)
+  int nsplit, split_blocks;
+  float *part, *lse;  // [slot][split][n_heads][head_dim] normalised outputs, [slot][split][n_heads] log2 sums
+  // decode
+  int nh, nhb;  // kv heads of a workgroup's 16 columns, head blocks of a row
+  // chunk
+  const int* tiles;
+  int n_tiles, ncg;  // column groups of a (tile, kv head)
+};
+
+// 8 consecutive q values of a column as QP bf16 parts.
+template <int QP>
+__device__ inline void load_q8(const AttnArgs& a, int64_t at, bool valid, bf16v8_t* part) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (valid) {
+    if (a.q_bf16) {
+      const uint16_t* p = (const uint16_t*)a.q + at;
+      if (a.q_vec) {
+        const u32x4_t w = *(const u32x4_t*)p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[2 * i] = bf16lo(w[i]);
+          x[2 * i + 1] = bf16hi(w[i]);
+        }
+      } else {
+        for (int i = 0; i < 8; ++i) x[i] = bf16_to_f32(p[i]);
+      }
+    } else {
+      const float* p = (const float*)a.q + at;
+      if (a.q_vec) {
+        const float4 u = *(const float4*)p, v = *(const float4*)(p + 4);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+      } else {
+        for (int i = 0; i < 8; ++i) x[i] = p[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < QP; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __bf16 h = (__bf16)x[i];
+      part[k][i] = h;
+      x[i] -= (float)h;
+    }
+}
+
+// First dim of the 8 that lane group g holds in k step s.
+template <int HD>
+__device__ inline int q_dim(int s, int g) {
+  if constexpr (HD == 32) return 8 * g;
+  else return 64 * (s / 2) + 16 * g + 8 * (s & 1);
+}
+
+// A lane's K bytes of one product: HD / 4 consecutive-in-16 bytes.
+template <int HD>
+struct KRaw {
+  uint32_t w[HD / 16];
+};
+
+template <int HD>
+__device__ inline KRaw<HD> load_k(const uint8_t* p) {
+  KRaw<HD> r;
+  if constexpr (HD == 32) {
+    const u32x2_t w = __builtin_nontemporal_load((const u32x2_t*)p);
+    r.w[0] = w[0];
+    r.w[1] = w[1];
+  } else {
+#pragma unroll
+    for (int h = 0; h < HD / 64; ++h) {
+      const u32x4_t w = __builtin_nontemporal_load((const u32x4_t*)(p + 64 * h));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.w[4 * h + i] = w[i];
+    }
+  }
+  return r;
+}
+
+// 8 codes (two dwords) as bf16, times scale's power of two.
+__device__ inline bf16v8_t codes_bf16(uint32_t lo, uint32_t hi, float scale) {
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+  return bf16v8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+__device__ inline f16v8_t codes_f16(uint32_t lo, uint32_t hi) {
+  const f16v2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+  const f16v2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+  const f16v2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+  const f16v2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+  return f16v8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Maximum / sum over the four lanes of a column (lanes n, n + 16, n + 32, n + 48).
+__device__ inline float column_max(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ inline float column_sum(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ inline int column_max(int x) {
+  auto r = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
+  x = max((int)r[0], (int)r[1]);
+  r = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false);
+  return max((int)r[0], (int)r[1]);
+}
+
+__device__ inline void store_out4(const AttnArgs& a, int64_t at, const float* o) {
+  if (a.out_bf16) {
+    uint16_t* p = (uint16_t*)a.out + at;
+    const uint2 w = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    if (a.out_vec) {
+      *(uint2*)p = w;
+    } else {
+      p[0] = (uint16_t)w.x; p[1] = (uint16_t)(w.x >> 16);
+      p[2] = (uint16_t)w.y; p[3] = (uint16_t)(w.y >> 16);
+    }
+  } else {
+    float* p = (float*)a.out + at;
+    if (a.out_vec) {
+      *(float4*)p = make_float4(o[0], o[1], o[2], o[3]);
+    } else {
+      for (int i = 0; i < 4; ++i) p[i] = o[i];
+    }
+  }
+}
+
+__device__ inline unsigned byte_of(uint32_t w, int i) { return (w >> (8 * i)) & 0xFFu; }
+
+// Byte mask of dword d (tokens 4 d .. 4 d + 3) of a tile's first `valid` tokens.
+__device__ inline uint32_t token_mask(int valid, int d) {
+  const int n = min(max(valid - 4 * d, 0), 4);
+  return n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
+}
+
+__device__ inline u32x4_t keep(bool mine, u32x4_t w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = mine ? w[i] : 0u;
+  return w;
+}
+
+// Single rows.  A workgroup owns (row, 16 query heads, split); its waves take
+// the split's 64-token blocks in turn.  The 16 columns of the products are 16
+// different heads: with q zero outside a kv head's own columns the scores of
+// all kv heads accumulate into the same four registers per product, each head
+// in its column, so the softmax runs once for 16 heads with no lane idle; the
+// output does the same with P.
+template <int HD, int QP, int PP>
+__global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const AttnArgs a) {
+  constexpr int NK = HD / 32, ND = HD / 16, HB = 128 / HD;
+  constexpr int kPitch = HD + 4;
+  __shared__ float o_sh[kDecodeWaves][16][kPitch];
+  __shared__ float lse_sh[kDecodeWaves][16];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  int bid = blockIdx.x;
+  const int hb = bid % a.nhb;
+  bid /= a.nhb;
+  const int split = bid % a.nsplit, ri = bid / a.nsplit;
+  const int row = a.rows ? a.rows[ri] : ri;
+  const int kv = min(a.row_pos[row], a.max_tok - 1) + 1;  // keys 0 .. kv - 1, none when <= 0
+  const int* bt = a.bt + (a.row_bt ? a.row_bt[row] : row) * a.bt_stride;
+  // Columns: column n is query head h0 + n of kv head kh0 + n / group.
+  int kh0, nhe, h0, ncol;
+  if (a.group >= 16) {
+    const int sub = (a.group + 15) / 16;
+    kh0 = hb / sub;
+    nhe = 1;
+    h0 = kh0 * a.group + hb % sub * 16;
+    ncol = min(16, (kh0 + 1) * a.group - h0);
+  } else {
+    kh0 = hb * a.nh;
+    nhe = min(a.nh, a.c.kv_heads - kh0);
+    h0 = kh0 * a.group;
+    ncol = nhe * a.group;
+  }
+  const bool col_ok = n < ncol;
+  const int my = col_ok ? (a.group >= 16 ? 0 : n / a.group) : -1;
+  const int my_head = kh0 + max(my, 0);
+
+  bf16v8_t q[NK][QP];
+#pragma unroll
+  for (int s = 0; s < NK; ++s)
+    load_q8<QP>(a, (int64_t)row * a.ldq + (int64_t)(h0 + n) * HD + q_dim<HD>(s, g), col_ok, q[s]);
+
+  float m = kLowest, l = 0.f;
+  int E = 0;
+  f32x4_t O[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) O[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  const int nblk = kv > 0 ? (kv + kBlk - 1) / kBlk : 0;
+  const int b0 = split * a.split_blocks;
+  const int b1 = split == a.nsplit - 1 ? nblk : min(nblk, b0 + a.split_blocks);
+  const int tlast = (kv - 1) >> 4;
+  const int64_t codes = (int64_t)a.c.kv_heads * HD * kTile;
+  for (int b = b0 + wave; b < b1; b += kDecodeWaves) {
+    const int64_t ko = tile_offset(a.c, bt, min(4 * b + (n >> 2), tlast));
+    const int64_t vo = tile_offset(a.c, bt, min(4 * b + g, tlast));
+    const uint8_t* kp = a.c.k + ko + (n & 3) * HD + (HD == 32 ? 8 : 16) * g;
+    const uint8_t* vp = a.c.v + vo + n * kTile;
+    const u32x4_t kb = *(const u32x4_t*)(a.c.k + vo + codes + my_head * kTile);  // tile g's K bytes of the column's head
+    u32x4_t vb = *(const u32x4_t*)(a.c.v + vo + codes + my_head * kTile);
+    f32x4_t S[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) S[p] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int hh = 0; hh < nhe; hh += HB) {
+      KRaw<HD> raw[HB][4];
+#pragma unroll
+      for (int j = 0; j < HB; ++j) {
+        const uint8_t* hp = kp + (int64_t)(kh0 + min(hh + j, nhe - 1)) * HD * kTile;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) raw[j][p] = load_k<HD>(hp + 4 * p * HD);
+      }
+#pragma unroll
+      for (int j = 0; j < HB; ++j) {
+        const bool mine = my == hh + j;
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+          bf16v8_t qm[QP];
+#pragma unroll
+          for (int k = 0; k < QP; ++k) qm[k] = __builtin_bit_cast(bf16v8_t, keep(mine, __builtin_bit_cast(u32x4_t, q[s][k])));
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const bf16v8_t kf = codes_bf16(raw[j][p].w[2 * s], raw[j][p].w[2 * s + 1], 1.f);
+#pragma unroll
+            for (int k = 0; k < QP; ++k) S[p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qm[k], S[p], 0, 0, 0);
+          }
+        }
+      }
+    }
+    const int valid = min(max(kv - (b * kBlk + g * kTile), 0), kTile);  // tokens of tile g inside the row
+    const bool tail = (b + 1) * kBlk > kv;
+    float top = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = S[p][i] * pow2_of_byte(byte_of(kb[p], i)) * a.qscale;
+        if (tail && 4 * p + i >= valid) x = -INFINITY;
+        S[p][i] = x;
+        top = fmaxf(top, x);
+      }
+    if (tail) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) vb[d] &= token_mask(valid, d);
+    }
+    int bmax = 0;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bmax = max(bmax, (int)byte_of(vb[d], i));
+    if (__ballot(bmax == kBadByte)) {  // a V slice of NaN: its columns' sums become NaN
+      bmax = 0;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if ((int)byte_of(vb[d], i) == kBadByte) {
+            if (col_ok) l = NAN;
+            vb[d] &= ~(0xFFu << (8 * i));
+          }
+          bmax = max(bmax, (int)byte_of(vb[d], i));
+        }
+    }
+    if (__ballot(top > m + 7.f || bmax > E)) {
+      const float m1 = fmaxf(m, column_max(top));
+      const int E1 = max(E, column_max(bmax));
+      const float r = fast_exp2(m - m1);
+      l *= r;
+      const float ro = ldexpf(r, E - E1);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) O[i] *= ro;
+      m = m1;
+      E = E1;
+    }
+    // p = 2^(s - m + 8), and P' = p * 2^(byte - E) in f16 parts.
+    f16v8_t P[2][PP];
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = fast_exp2(S[p][i] - m + 8.f);
+        l += e;
+        float x = ldexpf(e, (int)byte_of(vb[p], i) - E);
+#pragma unroll
+        for (int k = 0; k < PP; ++k) {
+          const _Float16 h = (_Float16)x;
+          P[p / 2][k][4 * (p & 1) + i] = h;
+          x -= (float)h;
+        }
+      }
+    const uint32_t vm[4] = {token_mask(valid, 0), token_mask(valid, 1), token_mask(valid, 2), token_mask(valid, 3)};
+    for (int hh = 0; hh < nhe; hh += HB) {
+      u32x4_t raw[HB][ND];
+#pragma unroll
+      for (int j = 0; j < HB; ++j) {
+        const uint8_t* hp = vp + (int64_t)(kh0 + min(hh + j, nhe - 1)) * HD * kTile;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) raw[j][i] = __builtin_nontemporal_load((const u32x4_t*)(hp + i * kTile * kTile));
+      }
+      if (tail) {  // a slot past the row may hold anything
+#pragma unroll
+        for (int j = 0; j < HB; ++j)
+#pragma unroll
+          for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) raw[j][i][d] &= vm[d];
+      }
+#pragma unroll
+      for (int j = 0; j < HB; ++j) {
+        const bool mine = my == hh + j;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          f16v8_t pm[PP];
+#pragma unroll
+          for (int k = 0; k < PP; ++k) pm[k] = __builtin_bit_cast(f16v8_t, keep(mine, __builtin_bit_cast(u32x4_t, P[half][k])));
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            const f16v8_t vf = codes_f16(raw[j][i][2 * half], raw[j][i][2 * half + 1]);
+#pragma unroll
+            for (int k = 0; k < PP; ++k) O[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pm[k], O[i], 0, 0, 0);
+          }
+        }
+      }
+    }
+  }
+
+  // Each wave's normalised output and log2 sum, then the waves' weighted mean.
+  l = column_sum(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (g == 0) lse_sh[wave][n] = l == 0.f ? -INFINITY : m - 8.f + __log2f(l);
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o_sh[wave][n][16 * i + 4 * g + r] = ldexpf(O[i][r] * inv, E - 127);
+  __syncthreads();
+  for (int t = threadIdx.x; t < 16 * HD / 4; t += kDecodeWaves * 64) {
+    const int col = t / (HD / 4), d = t % (HD / 4) * 4;
+    if (col >= ncol) continue;
+    float top = -INFINITY;
+    for (int w = 0; w < kDecodeWaves; ++w) top = fmaxf(top, lse_sh[w][col]);
+    float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+    for (int w = 0; w < kDecodeWaves; ++w) {
+      const float lw = lse_sh[w][col];
+      if (lw == -INFINITY) continue;
+      const float f = fast_exp2(lw - top);
+      sum += f;
+      for (int i = 0; i < 4; ++i) o[i] += f * o_sh[w][col][d + i];
+    }
+    const float norm = sum == 0.f ? 0.f : 1.f / sum;
+    for (int i = 0; i < 4; ++i) o[i] *= norm;
+    if (a.nsplit == 1) {
+      store_out4(a, (int64_t)row * a.ldo + (int64_t)(h0 + col) * HD + d, o);
+    } else {
+      const int64_t at = ((int64_t)ri * a.nsplit + split) * a.n_heads + h0 + col;
+      *(float4*)(a.part + at * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+      if (d == 0) a.lse[at] = sum == 0.f ? -INFINITY : top + __log2f(sum);
+    }
+  }
+}
+
+// Chunks.  A wave owns 16 CT columns of one (tile, kv head): column c is row c /
+// group of the tile and query head c % group of the kv head's group.  K and V
+// go from the cache through registers only; the waves of a workgroup are
+// independent.
+template <int HD, int CT, int QP, int PP>
+__global__ __launch_bounds__(kChunkWaves * 64) void kv8_chunk_kernel(const AttnArgs a) {
+  constexpr int NK = HD / 32, ND = HD / 16;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  int64_t unit = (int64_t)blockIdx.x * kChunkWaves + (threadIdx.x >> 6);
+  const int cg = (int)(unit % a.ncg);
+  unit /= a.ncg;
+  const int kh = (int)(unit % a.c.kv_heads);
+  unit /= a.c.kv_heads;
+  const int split = (int)(unit % a.nsplit);
+  const int64_t tile = unit / a.nsplit;
+  if (tile >= a.n_tiles) return;
+  const int row0 = a.tiles[4 * tile], nv = min(a.tiles[4 * tile + 1], CBIS_PREFILL_TILE_ROWS),
+            btr = a.tiles[4 * tile + 2], pos0 = a.tiles[4 * tile + 3];
+  const int c0 = cg * 16 * CT, cols = nv * a.group;
+  if (c0 >= cols) return;
+  const int* bt = a.bt + (int64_t)btr * a.bt_stride;
+  const int last_pos = min(pos0 + (min(c0 + 16 * CT, cols) - 1) / a.group, a.max_tok - 1);
+  const int first_pos = pos0 + c0 / a.group;
+  int pos[CT];
+  bf16v8_t q[CT][NK][QP];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = c0 + 16 * ct + n, t = c / a.group, head = kh * a.group + c % a.group;
+    const bool ok = c < cols;
+    pos[ct] = ok ? min(pos0 + t, a.max_tok - 1) : -1;
+#pragma unroll
+    for (int s = 0; s < NK; ++s)
+      load_q8<QP>(a, (int64_t)(row0 + t) * a.ldq + (int64_t)head * HD + q_dim<HD>(s, g), ok, q[ct][s]);
+  }
+  float m[CT], l[CT];
+  int E = 0;
+  f32x4_t O[ND][CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = kLowest;
+    l[ct] = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) O[i][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  const int kv = last_pos + 1;
+  const int nblk = kv > 0 ? (kv + kBlk - 1) / kBlk : 0;
+  const int b0 = split * a.split_blocks;
+  const int b1 = split == a.nsplit - 1 ? nblk : min(nblk, b0 + a.split_blocks);
+  const int tlast = (kv - 1) >> 4;
+  const int64_t codes = (int64_t)a.c.kv_heads * HD * kTile;
+  const int64_t head_codes = (int64_t)kh * HD * kTile;
+  for (int b = b0; b < b1; ++b) {
+    const int64_t ko = tile_offset(a.c, bt, min(4 * b + (n >> 2), tlast));
+    const int64_t vo = tile_offset(a.c, bt, min(4 * b + g, tlast));
+    const uint8_t* kp = a.c.k + ko + head_codes + (n & 3) * HD + (HD == 32 ? 8 : 16) * g;
+    const uint8_t* vp = a.c.v + vo + head_codes + n * kTile;
+    const u32x4_t kb = *(const u32x4_t*)(a.c.k + ko + codes + kh * kTile);
+    u32x4_t vb = *(const u32x4_t*)(a.c.v + vo + codes + kh * kTile);
+    KRaw<HD> kraw[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) kraw[p] = load_k<HD>(kp + 4 * p * HD);
+    u32x4_t vraw[ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) vraw[i] = *(const u32x4_t*)(vp + i * kTile * kTile);
+    f32x4_t S[4][CT];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const float ks = pow2_of_byte((kb[p] >> (8 * (n & 3))) & 0xFFu);  // 255: NaN scores
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) S[p][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < NK; ++s) {
+        const bf16v8_t kf = codes_bf16(kraw[p].w[2 * s], kraw[p].w[2 * s + 1], ks);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int k = 0; k < QP; ++k)
+            S[p][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[ct][s][k], S[p][ct], 0, 0, 0);
+      }
+    }
+    const int t0 = b * kBlk + g * kTile;  // first token of the lane's tile
+    if ((b + 1) * kBlk > first_pos + 1) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            if (t0 + 4 * p + i > pos[ct]) S[p][ct][i] = -INFINITY;
+    }
+    if ((b + 1) * kBlk > kv) {  // a slot past the last key may hold anything
+      const int valid = min(max(kv - t0, 0), kTile);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const uint32_t mask = token_mask(valid, d);
+        vb[d] &= mask;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) vraw[i][d] &= mask;
+      }
+    }
+    int bmax = 0;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bmax = max(bmax, (int)byte_of(vb[d], i));
+    if (__ballot(bmax == kBadByte)) {  // a V slice of NaN: the sums of the columns that see it become NaN
+      bmax = 0;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if ((int)byte_of(vb[d], i) == kBadByte) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+              if (t0 + 4 * d + i <= pos[ct]) l[ct] = NAN;
+            vb[d] &= ~(0xFFu << (8 * i));
+          }
+          bmax = max(bmax, (int)byte_of(vb[d], i));
+        }
+    }
+    float top[CT];
+    bool grow = bmax > E;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      top[ct] = -INFINITY;
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[ct] = fmaxf(top[ct], S[p][ct][i]);
+      top[ct] *= a.qscale;
+      grow |= top[ct] > m[ct] + 7.f;
+    }
+    if (__ballot(grow)) {
+      int E1 = max(E, column_max(bmax));
+      E1 = __builtin_amdgcn_readfirstlane(E1);  // tile g's bytes are the same in all its lanes
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const float m1 = fmaxf(m[ct], column_max(top[ct]));
+        const float r = fast_exp2(m[ct] - m1);
+        l[ct] *= r;
+        const float ro = ldexpf(r, E - E1);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) O[i][ct] *= ro;
+        m[ct] = m1;
+      }
+      E = E1;
+    }
+    // V as code * 2^(byte - E + 6) in f16 (at most 448 * 64), P as 2^(s - m + 8).
+    f16v8_t vs[2];
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        vs[d / 2][4 * (d & 1) + i] = (_Float16)ldexpf(1.f, (int)byte_of(vb[d], i) - E + 6);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      f16v8_t P[CT][PP];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float e = fast_exp2(S[2 * half + j / 4][ct][j & 3] * a.qscale - (m[ct] - 8.f));
+          l[ct] += e;
+          float x = e;
+#pragma unroll
+          for (int k = 0; k < PP; ++k) {
+            const _Float16 h = (_Float16)x;
+            P[ct][k][j] = h;
+            x -= (float)h;
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        const f16v8_t vf = codes_f16(vraw[i][2 * half], vraw[i][2 * half + 1]) * vs[half];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int k = 0; k < PP; ++k)
+            O[i][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, P[ct][k], O[i][ct], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = c0 + 16 * ct + n, t = c / a.group, head = kh * a.group + c % a.group;
+    const float sum = column_sum(l[ct]);
+    if (c >= cols) continue;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t at = ((tile * CBIS_PREFILL_TILE_ROWS + t) * a.nsplit + split) * a.n_heads + head;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      float o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = ldexpf(O[i][ct][r] * inv, E - 133);
+      const int d = 16 * i + 4 * g;
+      if (a.nsplit == 1) store_out4(a, (int64_t)(row0 + t) * a.ldo + (int64_t)head * HD + d, o);
+      else *(float4*)(a.part + at * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+    }
+    if (a.nsplit > 1 && g == 0) a.lse[at] = sum == 0.f ? -INFINITY : m[ct] - 8.f + __log2f(sum);
+  }
+}
+
+// The splits of a row's head joined: the mean of their outputs weighted by
+// their sums.  One thread per 4 dims.  A slot is a decode row or a tile's row.
+__global__ __launch_bounds__(256) void kv8_merge_kernel(const AttnArgs a, int64_t slots) {
+  const int HD = a.c.head_dim, q4 = HD / 4;
+  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int d = (int)(gid % q4) * 4;
+  const int64_t sh = gid / q4;
+  const int head = (int)(sh % a.n_heads);
+  const int64_t slot = sh / a.n_heads;
+  if (slot >= slots) return;
+  int64_t row;
+  if (a.tiles) {
+    const int64_t tile = slot / CBIS_PREFILL_TILE_ROWS;
+    const int t = (int)(slot % CBIS_PREFILL_TILE_ROWS);
+    if (t >= a.tiles[4 * tile + 1]) return;
+    row = (int64_t)a.tiles[4 * tile] + t;
+  } else {
+    row = a.rows ? a.rows[slot] : slot;
+  }
+  const int64_t first = slot * a.nsplit * a.n_heads + head;
+  float top = -INFINITY;
+  for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, a.lse[first + (int64_t)s * a.n_heads]);
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) {
+    const int64_t at = first + (int64_t)s * a.n_heads;
+    const float ls = a.lse[at];
+    if (ls == -INFINITY) continue;  // nothing was written for it
+    const float f = fast_exp2(ls - top);
+    sum += f;
+    const float4 x = *(const float4*)(a.part + at * HD + d);
+    o[0] += f * x.x; o[1] += f * x.y; o[2] += f * x.z; o[3] += f * x.w;
+  }
+  const float norm = sum == 0.f ? 0.f : 1.f / sum;
+  for (int i = 0; i < 4; ++i) o[i] *= norm;
+  store_out4(a, row * a.ldo + (int64_t)head * HD + d, o);
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+bool geometry_ok(int kv_heads, int head_dim, int page_size) {
+  return kv_heads > 0 && (head_dim == 32 || head_dim == 64 || head_dim == 128) && page_size >= kTile &&
+         (page_size & (page_size - 1)) == 0;
+}
+
+int make_pages(const cbis_kv8_cache* c, Pages* p, const char* who) {
+  CBIS_REQUIRE(c, CBIS_ERR_INVALID, "%s: null cache", who);
+  CBIS_REQUIRE(c->n_kv_heads > 0 && c->num_pages > 0, CBIS_ERR_INVALID, "%s: n_kv_heads %d, num_pages %d", who,
+               c->n_kv_heads, c->num_pages);
+  CBIS_REQUIRE(geometry_ok(c->n_kv_heads, c->head_dim, c->page_size), CBIS_ERR_UNSUPPORTED,
+               "%s: head_dim %d (32, 64 or 128), page_size %d (a power of two, at least 16)", who, c->head_dim,
+               c->page_size);
+  CBIS_REQUIRE(c->k_pool && c->v_pool && (((uintptr_t)c->k_pool | (uintptr_t)c->v_pool) & 15u) == 0, CBIS_ERR_INVALID,
+               "%s: the pools must be 16-byte aligned device pointers", who);
+  p->k = (uint8_t*)c->k_pool;
+  p->v = (uint8_t*)c->v_pool;
+  p->num_pages = c->num_pages;
+  p->page_size = c->page_size;
+  p->tshift = 0;
+  while ((kTile << p->tshift) < c->page_size) ++p->tshift;
+  p->kv_heads = c->n_kv_heads;
+  p->head_dim = c->head_dim;
+  p->tile_bytes = (int64_t)kTile * c->n_kv_heads * (c->head_dim + 1);
+  return CBIS_OK;
+}
+
+template <typename T, int HD>
+void rows_launch_hd(bool gather, bool vec, const RowsArgs& a, unsigned grid, hipStream_t s) {
+  if (gather) {
+    if (vec) kv8_gather_kernel<T, HD, true><<<grid, 256, 0, s>>>(a);
+    else kv8_gather_kernel<T, HD, false><<<grid, 256, 0, s>>>(a);
+  } else {
+    if (vec) kv8_scatter_kernel<T, HD, true><<<grid, 256, 0, s>>>(a);
+    else kv8_scatter_kernel<T, HD, false><<<grid, 256, 0, s>>>(a);
+  }
+}
+
+template <typename T>
+void rows_launch(bool gather, bool vec, const RowsArgs& a, unsigned grid, hipStream_t s) {
+  if (a.c.head_dim == 32) rows_launch_hd<T, 32>(gather, vec, a, grid, s);
+  else if (a.c.head_dim == 64) rows_launch_hd<T, 64>(gather, vec, a, grid, s);
+  else rows_launch_hd<T, 128>(gather, vec, a, grid, s);
+}
+
+int kv8_rows(bool gather, const cbis_kv8_cache* c, int n_rows, int dtype, const void* K, int64_t ldk, const void* V,
+             int64_t ldv, const int* page, const int* offset, hipStream_t s, const char* who) {
+  RowsArgs a = {};
+  const int rc = make_pages(c, &a.c, who);
+  if (rc) return rc;
+  CBIS_REQUIRE(n_rows >= 0, CBIS_ERR_INVALID, "%s: n_rows < 0", who);
+  CBIS_REQUIRE(dtype == CBIS_F32 || dtype == CBIS_BF16, CBIS_ERR_UNSUPPORTED, "%s: dtype %d (fp32 or bf16)", who, dtype);
+  if (n_rows == 0) return CBIS_OK;
+  const int64_t width = (int64_t)c->n_kv_heads * c->head_dim;
+  const size_t es = dtype == CBIS_F32 ? 4 : 2;
+  CBIS_REQUIRE(K && V && page && offset, CBIS_ERR_INVALID, "%s: null pointer", who);
+  CBIS_REQUIRE(ldk >= width && ldv >= width, CBIS_ERR_INVALID, "%s: row strides %lld, %lld below the row's %lld elements",
+               who, (long long)ldk, (long long)ldv, (long long)width);
+  CBIS_REQUIRE((((uintptr_t)K | (uintptr_t)V) & (es - 1)) == 0 && (((uintptr_t)page | (uintptr_t)offset) & 3u) == 0,
+               CBIS_ERR_INVALID, "%s: misaligned pointer", who);
+  a.n_rows = n_rows;
+  a.k = K;
+  a.v = V;
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.page = page;
+  a.offset = offset;
+  const bool vec = (((uintptr_t)K | (uintptr_t)V | (uintptr_t)(ldk * es) | (uintptr_t)(ldv * es)) & 15u) == 0;
+  const int64_t threads = (int64_t)n_rows * 2 * width / (16 / (int64_t)es);
+  CBIS_REQUIRE(cdiv(threads, 256) < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
+  const unsigned grid = (unsigned)cdiv(threads, 256);
+  if (dtype == CBIS_F32) rows_launch<float>(gather, vec, a, grid, s);
+  else rows_launch<uint16_t>(gather, vec, a, grid, s);
+  return check_launch(who);
+}
+
+// Sizes that both the workspace queries and the launches go by.
+struct Plan {
+  int nsplit = 1, split_blocks = 1 << 24;
+  int nh = 1, nhb = 1;   // decode
+  int ct = 2, ncg = 1;   // chunk
+  int64_t slots = 0;     // rows (or tile rows) of the partials
+  size_t bytes = 0;
+};
+
+bool heads_ok(const cbis_kv8_attn_desc* d) {
+  return d && geometry_ok(d->cache.n_kv_heads, d->cache.head_dim, d->cache.page_size) && d->n_heads > 0 &&
+         d->n_heads % d->cache.n_kv_heads == 0;
+}
+
+int64_t table_tokens(const cbis_kv8_attn_desc* d) {
+  return std::min<int64_t>(std::max<int64_t>(d->bt_stride, 0), (1 << 30) / d->cache.page_size) * d->cache.page_size;
+}
+
+// `units`: workgroups (or waves) of one split; `want`: how many the GPU takes.
+void plan_split(const cbis_kv8_attn_desc* d, int64_t units, int64_t want, int min_blocks, Plan* p) {
+  int64_t tok = table_tokens(d);
+  if (d->max_kv_len > 0) tok = std::min<int64_t>(tok, d->max_kv_len);
+  const int64_t blocks = std::max<int64_t>(1, cdiv(tok, kBlk));
+  int64_t per;
+  if (d->split_tokens > 0) {
+    per = cdiv(d->split_tokens, kBlk);
+  } else {
+    const int64_t n = std::max<int64_t>(1, want / std::max<int64_t>(1, units));
+    per = std::max<int64_t>(cdiv(blocks, n), min_blocks);
+  }
+  p->nsplit = (int)std::min<int64_t>(cdiv(blocks, per), 1 << 15);
+  p->split_blocks = (int)per;
+  if (p->nsplit > 1) p->bytes = (size_t)p->slots * p->nsplit * d->n_heads * (d->cache.head_dim + 1) * 4;
+}
+
+Plan plan_decode(const cbis_kv8_attn_desc* d) {
+  Plan p;
+  const int group = d->n_heads / d->cache.n_kv_heads;
+  if (group >= 16) {
+    p.nhb = d->cache.n_kv_heads * ((group + 15) / 16);
+  } else {
+    p.nh = std::min(16 / group, d->cache.n_kv_heads);
+    p.nhb = (d->cache.n_kv_heads + p.nh - 1) / p.nh;
+  }
+  p.slots = std::max(d->n_rows, 0);
+  plan_split(d, p.slots * p.nhb, 512, kDecodeWaves, &p);
+  return p;
+}
+
+Plan plan_chunk(const cbis_kv8_attn_desc* d, int n_tiles) {
+  Plan p;
+  const int group = d->n_heads / d->cache.n_kv_heads;
+  p.ct = 2;
+  p.ncg = (CBIS_PREFILL_TILE_ROWS * group + 16 * p.ct - 1) / (16 * p.ct);
+  p.slots = (int64_t)std::max(n_tiles, 0) * CBIS_PREFILL_TILE_ROWS;
+  plan_split(d, (int64_t)std::max(n_tiles, 0) * d->cache.n_kv_heads * p.ncg, 2048, 8, &p);
+  return p;
+}
+
+int attn_args(const cbis_kv8_attn_desc* d, AttnArgs* a, const char* who) {
+  CBIS_REQUIRE(d, CBIS_ERR_INVALID, "%s: null descriptor", who);
+  const int rc = make_pages(&d->cache, &a->c, who);
+  if (rc) return rc;
+  CBIS_REQUIRE(d->n_heads > 0 && d->n_heads % d->cache.n_kv_heads == 0, CBIS_ERR_INVALID,
+               "%s: n_heads %d must be a multiple of n_kv_heads %d", who, d->n_heads, d->cache.n_kv_heads);
+  CBIS_REQUIRE((d->q_dtype == CBIS_F32 || d->q_dtype == CBIS_BF16) && (d->out_dtype == CBIS_F32 || d->out_dtype == CBIS_BF16),
+               CBIS_ERR_UNSUPPORTED, "%s: q dtype %d, out dtype %d (fp32 or bf16)", who, d->q_dtype, d->out_dtype);
+  CBIS_REQUIRE(d->split_tokens >= 0 && d->split_tokens % kBlk == 0, CBIS_ERR_INVALID,
+               "%s: split_tokens %d must be a multiple of %d, or 0", who, d->split_tokens, kBlk);
+  CBIS_REQUIRE(d->max_kv_len >= 0, CBIS_ERR_INVALID, "%s: max_kv_len < 0", who);
+  const int64_t width = (int64_t)d->n_heads * d->cache.head_dim;
+  CBIS_REQUIRE(d->q && d->out && d->block_table, CBIS_ERR_INVALID, "%s: null pointer", who);
+  CBIS_REQUIRE(d->ldq >= width && d->ldo >= width && d->bt_stride > 0, CBIS_ERR_INVALID,
+               "%s: row strides %lld, %lld below the row's %lld elements, or bt_stride %lld", who, (long long)d->ldq,
+               (long long)d->ldo, (long long)width, (long long)d->bt_stride);
+  const size_t qs = d->q_dtype == CBIS_F32 ? 4 : 2, os = d->out_dtype == CBIS_F32 ? 4 : 2;
+  CBIS_REQUIRE(((uintptr_t)d->q & (qs - 1)) == 0 && ((uintptr_t)d->out & (os - 1)) == 0 &&
+                   (((uintptr_t)d->block_table | (uintptr_t)d->rows | (uintptr_t)d->row_bt | (uintptr_t)d->row_pos) & 3u) == 0,
+               CBIS_ERR_INVALID, "%s: misaligned pointer", who);
+  a->n_heads = d->n_heads;
+  a->group = d->n_heads / d->cache.n_kv_heads;
+  a->q = d->q;
+  a->ldq = d->ldq;
+  a->q_bf16 = d->q_dtype == CBIS_BF16;
+  a->q_vec = (((uintptr_t)d->q | (uintptr_t)(d->ldq * qs)) & 15u) == 0;
+  a->bt = d->block_table;
+  a->bt_stride = d->bt_stride;
+  a->out = d->out;
+  a->ldo = d->ldo;
+  a->out_bf16 = d->out_dtype == CBIS_BF16;
+  a->out_vec = (((uintptr_t)d->out | (uintptr_t)(d->ldo * os)) & (4 * os - 1)) == 0;
+  a->max_tok = (int)table_tokens(d);
+  a->qscale = kLog2e / sqrtf((float)d->cache.head_dim);
+  return CBIS_OK;
+}
+
+int take_workspace(const cbis_kv8_attn_desc* d, const Plan& p, AttnArgs* a, const char* who) {
+  a->nsplit = p.nsplit;
+  a->split_blocks = p.split_blocks;
+  if (p.nsplit == 1) return CBIS_OK;
+  CBIS_REQUIRE(d->workspace && d->workspace_bytes >= p.bytes, CBIS_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", who, p.bytes, d->workspace ? d->workspace_bytes : (size_t)0);
+  CBIS_REQUIRE(((uintptr_t)d->workspace & 15u) == 0, CBIS_ERR_INVALID, "%s: workspace must be 16-byte aligned", who);
+  a->part = (float*)d->workspace;
+  a->lse = a->part + p.slots * p.nsplit * d->n_heads * d->cache.head_dim;
+  return CBIS_OK;
+}
+
+int merge(const AttnArgs& a, const Plan& p, hipStream_t s, const char* who) {
+  const int64_t threads = p.slots * a.n_heads * (a.c.head_dim / 4);
+  CBIS_REQUIRE(cdiv(threads, 256) < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
+  kv8_merge_kernel<<<(unsigned)cdiv(threads, 256), 256, 0, s>>>(a, p.slots);
+  return check_launch(who);
+}
+
+template <int QP, int PP>
+void decode_parts(const AttnArgs& a, unsigned grid, hipStream_t s) {
+  constexpr int T = kDecodeWaves * 64;
+  if (a.c.head_dim == 32) kv8_decode_kernel<32, QP, PP><<<grid, T, 0, s>>>(a);
+  else if (a.c.head_dim == 64) kv8_decode_kernel<64, QP, PP><<<grid, T, 0, s>>>(a);
+  else kv8_decode_kernel<128, QP, PP><<<grid, T, 0, s>>>(a);
+}
+
+template <int QP, int PP>
+void chunk_parts(const AttnArgs& a, unsigned grid, hipStream_t s) {
+  constexpr int T = kChunkWaves * 64;
+  if (a.c.head_dim == 32) kv8_chunk_kernel<32, 2, QP, PP><<<grid, T, 0, s>>>(a);
+  else if (a.c.head_dim == 64) kv8_chunk_kernel<64, 2, QP, PP><<<grid, T, 0, s>>>(a);
+  else kv8_chunk_kernel<128, 2, QP, PP><<<grid, T, 0, s>>>(a);
+}
+
+}  // namespace
+}  // namespace cbis
+
+using namespace cbis;
+
+extern "C" {
+
+size_t cbis_kv8_page_bytes(int n_kv_heads, int head_dim, int page_size) {
+  if (!geometry_ok(n_kv_heads, head_dim, page_size)) return 0;
+  return (size_t)page_size * n_kv_heads * (head_dim + 1);
+}
+
+int cbis_kv8_scatter(const cbis_kv8_cache* c, int n_rows, int src_dtype, const void* K, int64_t ldk, const void* V,
+                     int64_t ldv, const int* write_page, const int* write_offset, cbis_stream_t stream) {
+  return kv8_rows(false, c, n_rows, src_dtype, K, ldk, V, ldv, write_page, write_offset, (hipStream_t)stream,
+                  "cbis_kv8_scatter");
+}
+
+int cbis_kv8_gather(const cbis_kv8_cache* c, int n_rows, int dst_dtype, void* K, int64_t ldk, void* V, int64_t ldv,
+                    const int* read_page, const int* read_offset, cbis_stream_t stream) {
+  return kv8_rows(true, c, n_rows, dst_dtype, K, ldk, V, ldv, read_page, read_offset, (hipStream_t)stream,
+                  "cbis_kv8_gather");
+}
+
+size_t cbis_kv8_attention_workspace_size(const cbis_kv8_attn_desc* d) { return heads_ok(d) ? plan_decode(d).bytes : 0; }
+
+int cbis_kv8_attention(const cbis_kv8_attn_desc* d, cbis_stream_t stream) {
+  const char* who = "cbis_kv8_attention";
+  AttnArgs a = {};
+  int rc = attn_args(d, &a, who);
+  if (rc) return rc;
+  CBIS_REQUIRE(d->n_rows >= 0, CBIS_ERR_INVALID, "%s: n_rows < 0", who);
+  if (d->n_rows == 0) return CBIS_OK;
+  CBIS_REQUIRE(d->row_pos, CBIS_ERR_INVALID, "%s: null row_pos", who);
+  const Plan p = plan_decode(d);
+  if ((rc = take_workspace(d, p, &a, who))) return rc;
+  a.n_rows = d->n_rows;
+  a.rows = d->rows;
+  a.row_bt = d->row_bt;
+  a.row_pos = d->row_pos;
+  a.nh = p.nh;
+  a.nhb = p.nhb;
+  const int64_t grid = p.slots * p.nhb * p.nsplit;
+  CBIS_REQUIRE(grid < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
+  hipStream_t s = (hipStream_t)stream;
+  if (a.out_bf16) {
+    if (a.q_bf16) decode_parts<1, 1>(a, (unsigned)grid, s);
+    else decode_parts<2, 1>(a, (unsigned)grid, s);
+  } else {
+    if (a.q_bf16) decode_parts<1, 2>(a, (unsigned)grid, s);
+    else decode_parts<3, 2>(a, (unsigned)grid, s);
+  }
+  rc = check_launch(who);
+  return rc || p.nsplit == 1 ? rc : merge(a, p, s, who);
+}
+
+size_t cbis_kv8_chunk_attention_workspace_size(const cbis_kv8_attn_desc* d, int n_tiles) {
+  return heads_ok(d) ? plan_chunk(d, n_tiles).bytes : 0;
+}
+
+int cbis_kv8_chunk_attention(const cbis_kv8_attn_desc* d, int n_tiles, const int* tiles, cbis_stream_t stream) {
+  const char* who = "cbis_kv8_chunk_attention";
+  AttnArgs a = {};
+  int rc = attn_args(d, &a, who);
+  if (rc) return rc;
+  CBIS_REQUIRE(n_tiles >= 0, CBIS_ERR_INVALID, "%s: n_tiles < 0", who);
+  if (n_tiles == 0) return CBIS_OK;
+  CBIS_REQUIRE(tiles && ((uintptr_t)tiles & 15u) == 0, CBIS_ERR_INVALID,
+               "%s: tiles must be a 16-byte aligned device array [n_tiles][4]", who);
+  const Plan p = plan_chunk(d, n_tiles);
+  if ((rc = take_workspace(d, p, &a, who))) return rc;
+  a.tiles = tiles;
+  a.n_tiles = n_tiles;
+  a.ncg = p.ncg;
+  const int64_t grid = cdiv((int64_t)n_tiles * p.nsplit * d->cache.n_kv_heads * p.ncg, kChunkWaves);
+  CBIS_REQUIRE(grid < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
+  hipStream_t s = (hipStream_t)stream;
+  if (a.out_bf16) {
+    if (a.q_bf16) chunk_parts<1, 1>(a, (unsigned)grid, s);
+    else chunk_parts<2, 1>(a, (unsigned)grid, s);
+  } else {
+    if (a.q_bf16) chunk_parts<1, 2>(a, (unsigned)grid, s);
+    else chunk_parts<3, 2>(a, (unsigned)grid, s);
+  }
+  rc = check_launch(who);
+  return rc || p.nsplit == 1 ? rc : merge(a, p, s, who);
+}
+
+}  // extern "C"

@@ -301,6 +301,94 @@ int cbis_paged_chunk_attention(const cbis_attn_desc* d, int n_tiles, const int* 
 int cbis_paged_attention_mixed(const cbis_attn_desc* d, int n_tiles, const int* tiles, cbis_stream_t stream);
 
 /* ----------------------------------------------------------------------- */
+/* The 8-bit paged K/V cache (no reference counterpart: the reference's      */
+/* cache is fp32).                                                           */
+/* ----------------------------------------------------------------------- */
+
+/* Half of bf16's bytes.  The K (or V) slice of one token and kv head,
+ * x[0 .. head_dim), is held as OCP e4m3 codes c and one byte b: with e the
+ * least integer >= -126 such that max|x| <= 448 * 2^e, b = e + 127,
+ * c_i = x_i * 2^-e rounded to nearest even, and the value read back is
+ * c_i * 2^e, off by at most 2^-4 of x_i (2^-10 * 2^e where |x_i| < 2^(e-6)).
+ * A slice that holds a NaN or an infinity is kept as b = 255 and zero codes
+ * and reads back as NaN throughout; other slices are not touched by it.
+ *
+ * A page of page_size tokens is page_size / 16 tiles.  A K tile is codes
+ * [n_kv_heads][16][head_dim] then bytes [n_kv_heads][16]; a V tile is codes
+ * [n_kv_heads][head_dim][16] then bytes [n_kv_heads][16].  A pool is num_pages
+ * pages of cbis_kv8_page_bytes() each, so cbis_kv_pages_gather / _scatter
+ * move its pages like any other's.  Supported: head_dim 32, 64 or 128, page_size
+ * a power of two >= 16, any n_kv_heads. */
+typedef struct cbis_kv8_cache {
+  int n_kv_heads, head_dim, page_size;
+  int num_pages;
+  void* k_pool; /* 16-byte aligned */
+  void* v_pool;
+} cbis_kv8_cache;
+
+/* Bytes of one page of a K or V pool: page_size * n_kv_heads * (head_dim + 1);
+ * 0 for a geometry that is not supported. */
+size_t cbis_kv8_page_bytes(int n_kv_heads, int head_dim, int page_size);
+
+/* Quantises row r of K and V ([n_rows, n_kv_heads * head_dim], fp32 or bf16, row
+ * strides ldk / ldv elements) into slot (write_page[r], write_offset[r]): the
+ * quantising form of cbis_scatter_kv_to_cache.  A row whose page is outside
+ * [0, num_pages) or whose offset is outside [0, page_size) is skipped (a padded
+ * batch's idle rows: -1).  Two rows of one call must not share a slot. */
+int cbis_kv8_scatter(const cbis_kv8_cache* c, int n_rows, int src_dtype, const void* K, int64_t ldk, const void* V,
+                     int64_t ldv, const int* write_page, const int* write_offset, cbis_stream_t stream);
+
+/* The inverse: slot (read_page[r], read_offset[r]) as row r of K and V, fp32 or
+ * bf16 (exact in both but for values past the type's range).  Rows whose slot
+ * is outside the pools are left as they were. */
+int cbis_kv8_gather(const cbis_kv8_cache* c, int n_rows, int dst_dtype, void* K, int64_t ldk, void* V, int64_t ldv,
+                    const int* read_page, const int* read_offset, cbis_stream_t stream);
+
+typedef struct cbis_kv8_attn_desc {
+  cbis_kv8_cache cache;
+  int n_rows;             /* rows to process (entries of `rows`, or 0..n_rows-1) */
+  const int* rows;        /* [n_rows] row ids into q/out/row_pos/row_bt, or NULL */
+  int n_heads;            /* query heads, a multiple of n_kv_heads: query head h reads
+                             kv head h / (n_heads / n_kv_heads) */
+  int q_dtype;            /* CBIS_F32 or CBIS_BF16 */
+  const void* q;          /* [*, n_heads * head_dim], row stride ldq elements */
+  int64_t ldq;
+  const int* block_table; /* [*, bt_stride] physical page ids (clamped to the pool) */
+  int64_t bt_stride;
+  const int* row_bt;      /* row -> block_table row, or NULL (row r uses row r) */
+  const int* row_pos;     /* row -> query position; it attends to keys [0, pos] */
+  int out_dtype;          /* CBIS_F32 or CBIS_BF16 */
+  void* out;              /* [*, n_heads * head_dim], row stride ldo elements */
+  int64_t ldo;
+  int max_kv_len;         /* about the longest row's pos + 1: it sets how the keys are
+                             split, not which are read; 0 = bt_stride * page_size */
+  int split_tokens;       /* keys per split, a multiple of 64; 0 = automatic */
+  void* workspace;        /* fp32 partials when the keys are split; 16-byte aligned */
+  size_t workspace_bytes;
+} cbis_kv8_attn_desc;
+
+/* Bytes of workspace cbis_kv8_attention needs for this descriptor (0: none). */
+size_t cbis_kv8_attention_workspace_size(const cbis_kv8_attn_desc* d);
+
+/* out[r] = softmax(q[r] K^T / sqrt(head_dim)) V over the 8-bit cache, for any
+ * set of rows, each with its own length (the decode form).  A row with a negative
+ * position attends to nothing and comes out zero; keys past
+ * bt_stride * page_size are not read.  What a page's slots past the row's
+ * last key hold does not matter.  Sums and statistics are fp32; with a bf16 result fp32 q is
+ * used to 16 bits and the probabilities to 11, with an fp32 result q in full
+ * and the probabilities to 22. */
+int cbis_kv8_attention(const cbis_kv8_attn_desc* d, cbis_stream_t stream);
+
+/* The same for tiles of up to CBIS_PREFILL_TILE_ROWS consecutive rows of one
+ * sequence: tiles is a device array [n_tiles][4] of {first_row, n_valid_rows,
+ * block_table_row, first_position}, as cbis_paged_prefill_attention's with
+ * tile_pages = 0; row i of a tile has position first_position + i.  Rows of a
+ * tile past CBIS_PREFILL_TILE_ROWS are not computed.  n_rows, rows, row_bt and
+ * row_pos are ignored. */
+size_t cbis_kv8_chunk_attention_workspace_size(const cbis_kv8_attn_desc* d, int n_tiles);
+int cbis_kv8_chunk_attention(const cbis_kv8_attn_desc* d, int n_tiles, const int* tiles, cbis_stream_t stream);
+
+/* ----------------------------------------------------------------------- */
 /* Row ops.                                                                  */
 /* ----------------------------------------------------------------------- */
 
