@@ -63,8 +63,21 @@ __device__ inline int64_t tile_offset(const Pages& c, const int* __restrict__ bt
 __device__ inline float pow2_of_byte(unsigned b) { return __uint_as_float(b << 23); }
 
 // ---------------------------------------------------------------------------
-// Write: one group of lanes per slice (row, K | V, head), 16 bytes of input
-// per lane.  HBM-bound; see the launch for its figures.
+// Rows in and out of their slots.
+//
+// A workgroup of 16 waves takes up to 16 rows of 256 (fp32) or 512 (bf16) columns
+// of K and of V, a row to a wave and 16 bytes of it to a lane.  Where the rows are the 16 tokens of one
+// cache tile (a prompt's rows) the V codes are turned in LDS, so that the tile's
+// dims are written and read in whole 16-byte pieces; other rows go slot by slot.
+// With a wave to a row and no more, the 16 bytes of a V dim came from up to 8
+// XCDs, each writing its own part of the line back.  HBM-bound on large calls,
+// by latency on small ones (so the waves share nothing they need not, and the
+// code is short: it is fetched anew by every launch).
+//
+// The rows are cut into groups where the tokens are: row r follows row r - 1 if
+// its slot is the next one of the same tile.  A window of 16 rows owns the runs
+// that start in it (which may end up to 15 rows behind it), and takes them in
+// groups of whole runs of at most 16 rows.
 // ---------------------------------------------------------------------------
 struct RowsArgs {
   Pages c;
@@ -72,144 +85,283 @@ struct RowsArgs {
   const void *k, *v;
   int64_t ldk, ldv;
   const int *page, *offset;
+  int parts;  // parts of 64 lanes' columns of a row
 };
 
 template <typename T>
-struct RowElems {
-  static constexpr int kPerLane = 16 / sizeof(T);
+constexpr int kLaneCols = 16 / sizeof(T);
+constexpr int kRowThreads = kTile * 64;
+
+// Rows need no more than their elements' alignment: gfx950 loads and stores
+// vectors at any address.
+typedef u32x4_t __attribute__((aligned(4))) u32x4_any_t;
+typedef u32x4_t __attribute__((aligned(2))) u32x4_half_t;
+
+__device__ inline bool slot_ok(const RowsArgs& a, int64_t row, int* page, int* off) {
+  if (row < 0 || row >= a.n_rows) return false;
+  *page = a.page[row];
+  *off = a.offset[row];
+  return (unsigned)*page < (unsigned)a.c.num_pages && (unsigned)*off < (unsigned)a.c.page_size;
+}
+
+// Lane i holds row window + i: its slot, and bit i whether it has one and
+// whether a run starts there (rows without a slot are runs of their own).
+struct RowSlots {
+  int page, off;
+  uint64_t starts, live;
 };
 
-template <typename T, bool kVec>
-__device__ inline void load_elems(const T* p, float* x) {
-  constexpr int N = RowElems<T>::kPerLane;
-  if constexpr (kVec) {
-    const u32x4_t w = __builtin_nontemporal_load((const u32x4_t*)p);
-    if constexpr (sizeof(T) == 4) {
+__device__ inline RowSlots row_slots(const RowsArgs& a, int64_t window, int lane) {
+  RowSlots r;
+  int p0 = 0, o0 = 0;
+  r.page = r.off = 0;
+  const bool live = slot_ok(a, window + lane, &r.page, &r.off), before = slot_ok(a, window + lane - 1, &p0, &o0);
+  const bool follows = live && before && r.page == p0 && r.off == o0 + 1 && (r.off & (kTile - 1)) != 0;
+  r.starts = __ballot(!follows);
+  r.live = __ballot(live);
+  return r;
+}
+
+// The end of the group that starts at row `at` of the window: whole runs of at
+// most 16 rows together, not past `end`.
+__device__ inline int group_end(uint64_t starts, int at, int end) {
+  const unsigned m = (unsigned)(starts >> (at + 1)) & 0xFFFFu;  // never 0: a run has at most 16 rows
+  return min(at + 32 - __clz((int)m), end);
+}
+
+// Transposes 4 x 4 bytes: dword i of the result holds byte i of each w.
+__device__ inline void transpose4(uint32_t* w) {
+  const uint32_t t0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), t1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+  const uint32_t u0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), u1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(u0, t0, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(u0, t0, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(u1, t1, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(u1, t1, 0x07060302u);
+}
+
+__device__ inline void load_row(const float* p, float* x) {
+  const u32x4_t w = __builtin_nontemporal_load((const u32x4_any_t*)p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
-    } else {
+  for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+}
+
+__device__ inline void load_row(const uint16_t* p, float* x) {
+  const u32x4_t w = __builtin_nontemporal_load((const u32x4_half_t*)p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = bf16lo(w[i]);
-        x[2 * i + 1] = bf16hi(w[i]);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if constexpr (sizeof(T) == 4) x[i] = ((const float*)p)[i];
-      else x[i] = bf16_to_f32(((const uint16_t*)p)[i]);
-    }
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = bf16lo(w[i]);
+    x[2 * i + 1] = bf16hi(w[i]);
   }
 }
 
-template <typename T, int HD, bool kVec>
-__global__ __launch_bounds__(256) void kv8_scatter_kernel(const RowsArgs a) {
-  constexpr int N = RowElems<T>::kPerLane, L = HD / N;
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int sub = (int)(gid % L);
-  const int64_t slice = gid / L;
-  const int H = a.c.kv_heads;
-  const int64_t row = slice / (2 * H);
-  if (row >= a.n_rows) return;  // whole groups only: a group is one slice
-  const int rest = (int)(slice % (2 * H));
-  const bool is_v = rest >= H;
-  const int head = is_v ? rest - H : rest;
-  const int page = a.page[row], off = a.offset[row];
-  if ((unsigned)page >= (unsigned)a.c.num_pages || (unsigned)off >= (unsigned)a.c.page_size) return;
-  const T* src = is_v ? (const T*)a.v + row * a.ldv : (const T*)a.k + row * a.ldk;
-  float x[N];
-  load_elems<T, kVec>(src + head * HD + sub * N, x);
-  unsigned top = 0;  // max |x| by its bits: NaN above infinity above every finite value
+__device__ inline void store_row(float* p, const float* x) {
+  __builtin_nontemporal_store(
+      u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])},
+      (u32x4_any_t*)p);
+}
+
+__device__ inline void store_row(uint16_t* p, const float* x) {
+  __builtin_nontemporal_store(u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                      pack_bf16x2(x[6], x[7])},
+                              (u32x4_half_t*)p);
+}
+
+// Maximum over aligned groups of L lanes (L = 4, 8, 16 or 32).
+template <int L>
+__device__ inline unsigned lanes_max(unsigned v) {
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));   // lane ^ 1
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));   // lane ^ 2
+  if constexpr (L >= 8) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));   // the other 4 of 8
+  if constexpr (L >= 16) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));  // of 16
+  if constexpr (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((unsigned)r[0], (unsigned)r[1]);
+  }
+  return v;
+}
+
+// A lane's N codes of a slice held by HD / N lanes, and the slice's scale byte.
+template <int HD, int N>
+__device__ inline void quantise(const float* x, uint32_t* w, int* byte) {
+  // max |x| by its bits: NaN above infinity above every finite value.
+  unsigned top = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-#pragma unroll
-  for (int m = 1; m < L; m *= 2) top = max(top, (unsigned)__shfl_xor((int)top, m, 64));
+  top = lanes_max<HD / N>(top);
   const bool bad = top >= 0x7F800000u;
   // max |x| = 1.m * 2^(E - 127) <= 448 * 2^e = 1.75 * 2^(8 + e): e + 127 = E - 8,
-  // one more where 1.m > 1.75.
-  const int byte = bad ? kBadByte : max(1, (int)(top >> 23) - 8 + ((top & 0x7FFFFFu) > 0x600000u));
-  const float inv = bad ? 0.f : pow2_of_byte((unsigned)(254 - byte));
-  uint32_t w[N / 4];
+  // one more where 1.m > 1.75 (where adding 0x1FFFFF to m carries).
+  const int b = max(1, (int)((top + 0x1FFFFFu) >> 23) - 8);
+  const float inv = pow2_of_byte((unsigned)(254 - b));
 #pragma unroll
-  for (int i = 0; i < N / 4; ++i) {
-    int d = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inv, x[4 * i + 1] * inv, 0, false);
-    d = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inv, x[4 * i + 3] * inv, d, true);
-    w[i] = bad ? 0u : (uint32_t)d;
+  for (int i = 0; i < N; i += 4) {
+    int d = __builtin_amdgcn_cvt_pk_fp8_f32(x[i] * inv, x[i + 1] * inv, 0, false);
+    d = __builtin_amdgcn_cvt_pk_fp8_f32(x[i + 2] * inv, x[i + 3] * inv, d, true);
+    w[i / 4] = bad ? 0u : (uint32_t)d;
   }
-  const int slot = off & (kTile - 1);
-  uint8_t* tile = (is_v ? a.c.v : a.c.k) + (((int64_t)page << a.c.tshift) + (off >> 4)) * a.c.tile_bytes;
-  if (is_v) {
-    uint8_t* dst = tile + ((int64_t)head * HD + sub * N) * kTile + slot;
-#pragma unroll
-    for (int i = 0; i < N; ++i) dst[i * kTile] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
-  } else {
-    uint8_t* dst = tile + ((int64_t)head * kTile + slot) * HD + sub * N;
-    if constexpr (N == 4) *(uint32_t*)dst = w[0];
-    else *(uint2*)dst = make_uint2(w[0], w[1]);
-  }
-  if (sub == 0) tile[(int64_t)H * HD * kTile + head * kTile + slot] = (uint8_t)byte;
+  *byte = bad ? kBadByte : b;
 }
 
-// ---------------------------------------------------------------------------
+template <int N>
+__device__ inline void values(const uint32_t* w, float scale, float* x) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i / 4], false);
+    const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i / 4], true);
+    x[i] = lo[0] * scale;
+    x[i + 1] = lo[1] * scale;
+    x[i + 2] = hi[0] * scale;
+    x[i + 3] = hi[1] * scale;
+  }
+}
+
+// What a workgroup of the row kernels works on.
+template <int HD, int N>
+struct RowPlace {
+  int wave, lane, part, col, head, dim, at, end;
+  int64_t window, codes;
+  bool col_ok;
+  RowSlots rs;
+  __device__ RowPlace(const RowsArgs& a) {
+    wave = threadIdx.x >> 6;
+    lane = threadIdx.x & 63;
+    window = (int64_t)(blockIdx.x / a.parts) * kTile;
+    part = (int)(blockIdx.x % a.parts);
+    col = (part * 64 + lane) * N;
+    col_ok = col < a.c.kv_heads * HD;
+    head = col / HD;
+    dim = col % HD;
+    codes = (int64_t)a.c.kv_heads * HD * kTile;
+    rs = row_slots(a, window, lane);
+    at = rs.starts & 0xFFFF ? __ffsll((unsigned long long)rs.starts) - 1 : 64;  // 64: the window owns no row
+    end = kTile + __ffsll((unsigned long long)(rs.starts >> kTile)) - 1;
+  }
+  // Whether rows at .. stop - 1 are a cache tile's 16 tokens.
+  __device__ bool whole(int stop) const {
+    return stop - at == kTile && ((rs.starts >> (at + 1)) & 0x7FFF) == 0 && (rs.live >> at & 1);
+  }
+  __device__ bool mine(int stop) const { return at + wave < stop && (rs.live >> (at + wave) & 1); }
+  // Offset of the tile that row at + i lies in, and its slot there.
+  __device__ int64_t tile(const RowsArgs& a, int i, int* slot) const {
+    const int page = __builtin_amdgcn_readlane(rs.page, at + i), off = __builtin_amdgcn_readlane(rs.off, at + i);
+    *slot = off & (kTile - 1);
+    return (((int64_t)page << a.c.tshift) + (off >> 4)) * a.c.tile_bytes;
+  }
+};
+
+template <typename T, int HD>
+__global__ __launch_bounds__(kRowThreads) void kv8_scatter_kernel(const RowsArgs a) {
+  constexpr int N = kLaneCols<T>, NW = N / 4;
+  __shared__ uint32_t turn[kTile][64 * NW];  // V codes of the group's rows, 4 columns to a dword
+  RowPlace<HD, N> r(a);
+  for (int stop; r.at < r.end; r.at = stop) {
+    stop = group_end(r.rs.starts, r.at, r.end);
+    const bool whole = r.whole(stop);
+    if (r.mine(stop)) {
+      const int64_t row = r.window + r.at + r.wave;
+      float xk[N] = {}, xv[N] = {};
+      if (r.col_ok) {
+        load_row((const T*)a.k + row * a.ldk + r.col, xk);
+        load_row((const T*)a.v + row * a.ldv + r.col, xv);
+      }
+      int slot, bk, bv;
+      const int64_t tile = r.tile(a, r.wave, &slot);
+      uint32_t wk[NW], wv[NW];
+      quantise<HD, N>(xk, wk, &bk);
+      quantise<HD, N>(xv, wv, &bv);
+      if (r.col_ok) {
+        uint8_t* dk = a.c.k + tile + ((int64_t)r.head * kTile + slot) * HD + r.dim;
+        if constexpr (NW == 1) *(uint32_t*)dk = wk[0];
+        else *(u32x2_t*)dk = u32x2_t{wk[0], wk[1]};
+        if (r.dim == 0) {
+          a.c.k[tile + r.codes + r.head * kTile + slot] = (uint8_t)bk;
+          a.c.v[tile + r.codes + r.head * kTile + slot] = (uint8_t)bv;
+        }
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < NW; ++i) turn[r.wave][r.lane * NW + i] = wv[i];
+        } else {
+          uint8_t* dv = a.c.v + tile + (int64_t)r.col * kTile + slot;
+#pragma unroll
+          for (int j = 0; j < N; ++j) dv[j * kTile] = (uint8_t)(wv[j / 4] >> (8 * (j & 3)));
+        }
+      }
+    }
+    if (whole) {
+      __syncthreads();
+      // Thread t of the first NW waves takes columns 4 t .. 4 t + 3 of the part.
+      const int col = r.part * 64 * N + 4 * (int)threadIdx.x;
+      if (r.wave < NW && col < a.c.kv_heads * HD) {
+        int slot;
+        uint8_t* dst = a.c.v + r.tile(a, 0, &slot) + (int64_t)col * kTile;
+        uint32_t w[kTile];
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) w[i] = turn[i][threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < kTile; i += 4) transpose4(w + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(u32x4_t*)(dst + j * kTile) = u32x4_t{w[j], w[4 + j], w[8 + j], w[12 + j]};
+      }
+      __syncthreads();
+    }
+  }
+}
+
 // Read back: the same groups the other way.
-// ---------------------------------------------------------------------------
-template <typename T, int HD, bool kVec>
-__global__ __launch_bounds__(256) void kv8_gather_kernel(const RowsArgs a) {
-  constexpr int N = RowElems<T>::kPerLane, L = HD / N;
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int sub = (int)(gid % L);
-  const int64_t slice = gid / L;
-  const int H = a.c.kv_heads;
-  const int64_t row = slice / (2 * H);
-  if (row >= a.n_rows) return;
-  const int rest = (int)(slice % (2 * H));
-  const bool is_v = rest >= H;
-  const int head = is_v ? rest - H : rest;
-  const int page = a.page[row], off = a.offset[row];
-  if ((unsigned)page >= (unsigned)a.c.num_pages || (unsigned)off >= (unsigned)a.c.page_size) return;
-  const int slot = off & (kTile - 1);
-  const uint8_t* tile = (is_v ? a.c.v : a.c.k) + (((int64_t)page << a.c.tshift) + (off >> 4)) * a.c.tile_bytes;
-  uint32_t w[N / 4];
-  if (is_v) {
-    const uint8_t* src = tile + ((int64_t)head * HD + sub * N) * kTile + slot;
+template <typename T, int HD>
+__global__ __launch_bounds__(kRowThreads) void kv8_gather_kernel(const RowsArgs a) {
+  constexpr int N = kLaneCols<T>, NW = N / 4;
+  __shared__ uint32_t turn[kTile][64 * NW];
+  RowPlace<HD, N> r(a);
+  for (int stop; r.at < r.end; r.at = stop) {
+    stop = group_end(r.rs.starts, r.at, r.end);
+    const bool whole = r.whole(stop);
+    if (whole) {
+      const int col = r.part * 64 * N + 4 * (int)threadIdx.x;
+      if (r.wave < NW && col < a.c.kv_heads * HD) {
+        int slot;
+        const uint8_t* src = a.c.v + r.tile(a, 0, &slot) + (int64_t)col * kTile;
+        uint32_t w[kTile];
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i)
-      w[i] = src[(4 * i) * kTile] | src[(4 * i + 1) * kTile] << 8 | src[(4 * i + 2) * kTile] << 16 |
-             (uint32_t)src[(4 * i + 3) * kTile] << 24;
-  } else {
-    const uint8_t* src = tile + ((int64_t)head * kTile + slot) * HD + sub * N;
+        for (int j = 0; j < 4; ++j) {
+          const u32x4_t v = *(const u32x4_t*)(src + j * kTile);
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) w[i] = ((const uint32_t*)src)[i];
-  }
-  const float scale = pow2_of_byte(tile[(int64_t)H * HD * kTile + head * kTile + slot]);
-  float x[N];
+          for (int i = 0; i < 4; ++i) w[4 * i + j] = v[i];
+        }
 #pragma unroll
-  for (int i = 0; i < N / 4; ++i) {
-    const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
-    const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-    x[4 * i] = lo[0] * scale;
-    x[4 * i + 1] = lo[1] * scale;
-    x[4 * i + 2] = hi[0] * scale;
-    x[4 * i + 3] = hi[1] * scale;
-  }
-  T* dst = (T*)(is_v ? a.v : a.k) + row * (is_v ? a.ldv : a.ldk) + head * HD + sub * N;
-  if constexpr (kVec) {
-    u32x4_t o;
-    if constexpr (sizeof(T) == 4) {
+        for (int i = 0; i < kTile; i += 4) transpose4(w + i);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = __float_as_uint(x[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+        for (int i = 0; i < kTile; ++i) turn[i][threadIdx.x] = w[i];
+      }
+      __syncthreads();
     }
-    __builtin_nontemporal_store(o, (u32x4_t*)dst);
-  } else {
+    if (r.mine(stop) && r.col_ok) {
+      int slot;
+      const int64_t tile = r.tile(a, r.wave, &slot);
+      const uint32_t* src = (const uint32_t*)(a.c.k + tile + ((int64_t)r.head * kTile + slot) * HD + r.dim);
+      uint32_t wk[NW], wv[NW];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if constexpr (sizeof(T) == 4) ((float*)dst)[i] = x[i];
-      else ((uint16_t*)dst)[i] = f32_to_bf16(x[i]);
+      for (int i = 0; i < NW; ++i) wk[i] = src[i];
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) wv[i] = turn[r.wave][r.lane * NW + i];
+      } else {
+        const uint8_t* sv = a.c.v + tile + (int64_t)r.col * kTile + slot;
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+          wv[i] = sv[4 * i * kTile] | sv[(4 * i + 1) * kTile] << 8 | sv[(4 * i + 2) * kTile] << 16 |
+                  (uint32_t)sv[(4 * i + 3) * kTile] << 24;
+      }
+      const float sk = pow2_of_byte(a.c.k[tile + r.codes + r.head * kTile + slot]);
+      const float sv = pow2_of_byte(a.c.v[tile + r.codes + r.head * kTile + slot]);
+      const int64_t row = r.window + r.at + r.wave;
+      float x[N];
+      values<N>(wk, sk, x);
+      store_row((T*)a.k + row * a.ldk + r.col, x);
+      values<N>(wv, sv, x);
+      store_row((T*)a.v + row * a.ldv + r.col, x);
     }
+    if (whole) __syncthreads();
   }
 }
 
@@ -888,22 +1040,17 @@ int make_pages(const cbis_kv8_cache* c, Pages* p, const char* who) {
   return CBIS_OK;
 }
 
-template <typename T, int HD>
-void rows_launch_hd(bool gather, bool vec, const RowsArgs& a, unsigned grid, hipStream_t s) {
-  if (gather) {
-    if (vec) kv8_gather_kernel<T, HD, true><<<grid, 256, 0, s>>>(a);
-    else kv8_gather_kernel<T, HD, false><<<grid, 256, 0, s>>>(a);
-  } else {
-    if (vec) kv8_scatter_kernel<T, HD, true><<<grid, 256, 0, s>>>(a);
-    else kv8_scatter_kernel<T, HD, false><<<grid, 256, 0, s>>>(a);
-  }
-}
-
 template <typename T>
-void rows_launch(bool gather, bool vec, const RowsArgs& a, unsigned grid, hipStream_t s) {
-  if (a.c.head_dim == 32) rows_launch_hd<T, 32>(gather, vec, a, grid, s);
-  else if (a.c.head_dim == 64) rows_launch_hd<T, 64>(gather, vec, a, grid, s);
-  else rows_launch_hd<T, 128>(gather, vec, a, grid, s);
+void rows_launch(bool gather, const RowsArgs& a, unsigned grid, hipStream_t s) {
+  if (gather) {
+    if (a.c.head_dim == 32) kv8_gather_kernel<T, 32><<<grid, kRowThreads, 0, s>>>(a);
+    else if (a.c.head_dim == 64) kv8_gather_kernel<T, 64><<<grid, kRowThreads, 0, s>>>(a);
+    else kv8_gather_kernel<T, 128><<<grid, kRowThreads, 0, s>>>(a);
+  } else {
+    if (a.c.head_dim == 32) kv8_scatter_kernel<T, 32><<<grid, kRowThreads, 0, s>>>(a);
+    else if (a.c.head_dim == 64) kv8_scatter_kernel<T, 64><<<grid, kRowThreads, 0, s>>>(a);
+    else kv8_scatter_kernel<T, 128><<<grid, kRowThreads, 0, s>>>(a);
+  }
 }
 
 int kv8_rows(bool gather, const cbis_kv8_cache* c, int n_rows, int dtype, const void* K, int64_t ldk, const void* V,
@@ -928,12 +1075,11 @@ int kv8_rows(bool gather, const cbis_kv8_cache* c, int n_rows, int dtype, const 
   a.ldv = ldv;
   a.page = page;
   a.offset = offset;
-  const bool vec = (((uintptr_t)K | (uintptr_t)V | (uintptr_t)(ldk * es) | (uintptr_t)(ldv * es)) & 15u) == 0;
-  const int64_t threads = (int64_t)n_rows * 2 * width / (16 / (int64_t)es);
-  CBIS_REQUIRE(cdiv(threads, 256) < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
-  const unsigned grid = (unsigned)cdiv(threads, 256);
-  if (dtype == CBIS_F32) rows_launch<float>(gather, vec, a, grid, s);
-  else rows_launch<uint16_t>(gather, vec, a, grid, s);
+  a.parts = (int)cdiv(width, 64 * (16 / (int64_t)es));
+  const int64_t grid = cdiv(n_rows, kTile) * a.parts;
+  CBIS_REQUIRE(grid < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
+  if (dtype == CBIS_F32) rows_launch<float>(gather, a, (unsigned)grid, s);
+  else rows_launch<uint16_t>(gather, a, (unsigned)grid, s);
   return check_launch(who);
 }
 
