@@ -38,7 +38,7 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 constexpr int kTile = 16;          // tokens of a cache tile
 constexpr int kBlk = 64;           // tokens a wave takes at a time: four tiles
 constexpr int kBadByte = 255;      // scale byte of a slice with a non-finite value
-constexpr int kDecodeWaves = 8;
+constexpr int kDecodeWaves = 8;   // of a workgroup, at most
 constexpr int kChunkWaves = 4;
 constexpr float kLowest = -3.3e38f;  // a running maximum before any score
 
@@ -402,7 +402,7 @@ struct AttnArgs {
   int nsplit, split_blocks;
   float *part, *lse;  // [slot][split][n_heads][head_dim] normalised outputs, [slot][split][n_heads] log2 sums
   // decode
-  int nh, nhb;  // kv heads of a workgroup's 16 columns, head blocks of a row
+  int nhb, tw;  // head blocks of a row, waves of a workgroup that share one
   // chunk
   const int* tiles;
   int n_tiles, ncg;  // column groups of a (tile, kv head)
@@ -552,43 +552,53 @@ __device__ inline u32x4_t keep(bool mine, u32x4_t w) {
   return w;
 }
 
-// Single rows.  A workgroup owns (row, 16 query heads, split); its waves take
-// the split's 64-token blocks in turn.  The 16 columns of the products are 16
-// different heads: with q zero outside a kv head's own columns the scores of
-// all kv heads accumulate into the same four registers per product, each head
-// in its column, so the softmax runs once for 16 heads with no lane idle; the
-// output does the same with P.
-template <int HD, int QP, int PP>
+// Single rows.  A workgroup owns (row, NH kv heads, split); its waves take the
+// split's 64-token blocks in turn.  The 16 columns of the products are the query
+// heads: with q zero outside a kv head's own columns the scores of the NH kv
+// heads accumulate into the same four registers per product, each head in its
+// column, so one softmax serves them all; the output does the same with P.
+//
+// Bound by HBM while enough bytes are in flight: a block's K and V are 32
+// registers of loads each (NH * HD = 128), the next block's K is loaded as soon
+// as this one's has been multiplied, V likewise, so that one of the two is
+// always on its way.  Page ids are read two blocks ahead, before the loads whose
+// arrival would otherwise have to be awaited with them.
+template <int HD, int NH, int QP, int PP>
 __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const AttnArgs a) {
-  constexpr int NK = HD / 32, ND = HD / 16, HB = 128 / HD;
+  constexpr int NK = HD / 32, ND = HD / 16;
   constexpr int kPitch = HD + 4;
-  __shared__ float o_sh[kDecodeWaves][16][kPitch];
-  __shared__ float lse_sh[kDecodeWaves][16];
+  extern __shared__ float o_sh[];  // [wave][16][kPitch], then lse_sh [wave][16]; none where tw is 1
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  // All rows' last splits first, their first ones at the end, where the short
+  // rows (behind the long ones, if the caller sorts them) fill the tail.  With a
+  // row's splits side by side the later (often empty) ones would fall on the
+  // same XCDs for every row: workgroup b runs on XCD b % 8.
+  // The waves are tw token parts of waves / tw head blocks.
+  const int waves = blockDim.x >> 6, hpw = waves / a.tw, groups = (a.nhb + hpw - 1) / hpw;
   int bid = blockIdx.x;
-  const int hb = bid % a.nhb;
-  bid /= a.nhb;
-  const int split = bid % a.nsplit, ri = bid / a.nsplit;
+  const int hb = bid % groups * hpw + wave / a.tw, tpart = wave % a.tw;
+  bid /= groups;
+  const int ri = bid % a.n_rows, split = a.nsplit - 1 - bid / a.n_rows;
   const int row = a.rows ? a.rows[ri] : ri;
   const int kv = min(a.row_pos[row], a.max_tok - 1) + 1;  // keys 0 .. kv - 1, none when <= 0
   const int* bt = a.bt + (a.row_bt ? a.row_bt[row] : row) * a.bt_stride;
-  // Columns: column n is query head h0 + n of kv head kh0 + n / group.
-  int kh0, nhe, h0, ncol;
-  if (a.group >= 16) {
+  // Columns: column n is query head h0 + n, of kv head kh0 + n / group (of kh0
+  // where a kv head has 16 or more).
+  int kh0, h0, ncol;
+  if (NH == 1 && a.group > 16) {
     const int sub = (a.group + 15) / 16;
     kh0 = hb / sub;
-    nhe = 1;
     h0 = kh0 * a.group + hb % sub * 16;
     ncol = min(16, (kh0 + 1) * a.group - h0);
   } else {
-    kh0 = hb * a.nh;
-    nhe = min(a.nh, a.c.kv_heads - kh0);
+    kh0 = hb * NH;
     h0 = kh0 * a.group;
-    ncol = nhe * a.group;
+    ncol = min(NH, a.c.kv_heads - kh0) * a.group;
   }
+  if (hb >= a.nhb) ncol = 0;
   const bool col_ok = n < ncol;
-  const int my = col_ok ? (a.group >= 16 ? 0 : n / a.group) : -1;
-  const int my_head = kh0 + max(my, 0);
+  const int my = !col_ok ? -1 : NH == 1 ? 0 : n / a.group;
+  const int my_head = min(kh0 + max(my, 0), a.c.kv_heads - 1);
 
   bf16v8_t q[NK][QP];
 #pragma unroll
@@ -602,31 +612,54 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
   for (int i = 0; i < ND; ++i) O[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
   const int nblk = kv > 0 ? (kv + kBlk - 1) / kBlk : 0;
-  const int b0 = split * a.split_blocks;
-  const int b1 = split == a.nsplit - 1 ? nblk : min(nblk, b0 + a.split_blocks);
+  const int b0 = split * a.split_blocks + tpart, step = a.tw;
+  const int b1 = ncol <= 0 ? 0 : split == a.nsplit - 1 ? nblk : min(nblk, (split + 1) * a.split_blocks);
   const int tlast = (kv - 1) >> 4;
   const int64_t codes = (int64_t)a.c.kv_heads * HD * kTile;
-  for (int b = b0 + wave; b < b1; b += kDecodeWaves) {
-    const int64_t ko = tile_offset(a.c, bt, min(4 * b + (n >> 2), tlast));
-    const int64_t vo = tile_offset(a.c, bt, min(4 * b + g, tlast));
-    const uint8_t* kp = a.c.k + ko + (n & 3) * HD + (HD == 32 ? 8 : 16) * g;
-    const uint8_t* vp = a.c.v + vo + n * kTile;
-    const u32x4_t kb = *(const u32x4_t*)(a.c.k + vo + codes + my_head * kTile);  // tile g's K bytes of the column's head
-    u32x4_t vb = *(const u32x4_t*)(a.c.v + vo + codes + my_head * kTile);
-    f32x4_t S[4];
+  // Lane offsets inside a tile; kv heads past the last one read the last.
+  const int k_lane = (n & 3) * HD + (HD == 32 ? 8 : 16) * g;
+  int64_t head_off[NH];
 #pragma unroll
-    for (int p = 0; p < 4; ++p) S[p] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int hh = 0; hh < nhe; hh += HB) {
-      KRaw<HD> raw[HB][4];
+  for (int j = 0; j < NH; ++j) head_off[j] = (int64_t)min(kh0 + j, a.c.kv_heads - 1) * HD * kTile;
+  const int64_t byte_off = codes + my_head * kTile;
+
+  KRaw<HD> kr[NH][4];
+  u32x4_t vr[NH][ND];
+  auto load_k_block = [&](int64_t tile) {
+    const uint8_t* p0 = a.c.k + tile + k_lane;
 #pragma unroll
-      for (int j = 0; j < HB; ++j) {
-        const uint8_t* hp = kp + (int64_t)(kh0 + min(hh + j, nhe - 1)) * HD * kTile;
+    for (int j = 0; j < NH; ++j)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) raw[j][p] = load_k<HD>(hp + 4 * p * HD);
-      }
+      for (int p = 0; p < 4; ++p) kr[j][p] = load_k<HD>(p0 + head_off[j] + 4 * p * HD);
+  };
+  auto load_v_block = [&](int64_t tile) {
+    const uint8_t* p0 = a.c.v + tile + n * kTile;
 #pragma unroll
-      for (int j = 0; j < HB; ++j) {
-        const bool mine = my == hh + j;
+    for (int j = 0; j < NH; ++j)
+#pragma unroll
+      for (int i = 0; i < ND; ++i) vr[j][i] = __builtin_nontemporal_load((const u32x4_t*)(p0 + head_off[j] + i * kTile * kTile));
+  };
+
+  if (b0 < b1) {
+    // Tiles of the block the K loads, and of the one the V loads, are at.
+    int64_t ko = tile_offset(a.c, bt, min(4 * b0 + (n >> 2), tlast));
+    int64_t vo = tile_offset(a.c, bt, min(4 * b0 + g, tlast));
+    int64_t ko1 = tile_offset(a.c, bt, min(4 * (b0 + step) + (n >> 2), tlast));
+    int64_t vo1 = tile_offset(a.c, bt, min(4 * (b0 + step) + g, tlast));
+    load_k_block(ko);
+    u32x4_t kb = *(const u32x4_t*)(a.c.k + vo + byte_off);  // tile g's scale bytes of the column's head
+    u32x4_t vb = *(const u32x4_t*)(a.c.v + vo + byte_off);
+    load_v_block(vo);
+    // Behind the last block the loads go to the row's last tile again.  They are
+    // not branched around: where loads may or may not have been issued, the wait
+    // for older ones would be for these too.
+    for (int b = b0; b < b1; b += step) {
+      f32x4_t S[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) S[p] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NH; ++j) {
+        const bool mine = NH == 1 || my == j;
 #pragma unroll
         for (int s = 0; s < NK; ++s) {
           bf16v8_t qm[QP];
@@ -634,94 +667,88 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
           for (int k = 0; k < QP; ++k) qm[k] = __builtin_bit_cast(bf16v8_t, keep(mine, __builtin_bit_cast(u32x4_t, q[s][k])));
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
-            const bf16v8_t kf = codes_bf16(raw[j][p].w[2 * s], raw[j][p].w[2 * s + 1], 1.f);
+            const bf16v8_t kf = codes_bf16(kr[j][p].w[2 * s], kr[j][p].w[2 * s + 1], 1.f);
 #pragma unroll
             for (int k = 0; k < QP; ++k) S[p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qm[k], S[p], 0, 0, 0);
           }
         }
       }
-    }
-    const int valid = min(max(kv - (b * kBlk + g * kTile), 0), kTile);  // tokens of tile g inside the row
-    const bool tail = (b + 1) * kBlk > kv;
-    float top = -INFINITY;
+      __builtin_amdgcn_sched_barrier(0);
+      load_k_block(ko1);
+      __builtin_amdgcn_sched_barrier(0);
+      const int valid = min(max(kv - (b * kBlk + g * kTile), 0), kTile);  // tokens of tile g inside the row
+      const bool tail = (b + 1) * kBlk > kv;
+      float top = -INFINITY;
 #pragma unroll
-    for (int p = 0; p < 4; ++p)
+      for (int p = 0; p < 4; ++p)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = S[p][i] * pow2_of_byte(byte_of(kb[p], i)) * a.qscale;
-        if (tail && 4 * p + i >= valid) x = -INFINITY;
-        S[p][i] = x;
-        top = fmaxf(top, x);
+        for (int i = 0; i < 4; ++i) {
+          float x = S[p][i] * (pow2_of_byte(byte_of(kb[p], i)) * a.qscale);
+          if (tail && 4 * p + i >= valid) x = -INFINITY;
+          S[p][i] = x;
+          top = fmaxf(top, x);
+        }
+      if (tail) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) vb[d] &= token_mask(valid, d);
       }
-    if (tail) {
-#pragma unroll
-      for (int d = 0; d < 4; ++d) vb[d] &= token_mask(valid, d);
-    }
-    int bmax = 0;
-#pragma unroll
-    for (int d = 0; d < 4; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) bmax = max(bmax, (int)byte_of(vb[d], i));
-    if (__ballot(bmax == kBadByte)) {  // a V slice of NaN: its columns' sums become NaN
-      bmax = 0;
+      int bmax = 0;
 #pragma unroll
       for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if ((int)byte_of(vb[d], i) == kBadByte) {
-            if (col_ok) l = NAN;
-            vb[d] &= ~(0xFFu << (8 * i));
+        for (int i = 0; i < 4; ++i) bmax = max(bmax, (int)byte_of(vb[d], i));
+      if (__ballot(bmax == kBadByte)) {  // a V slice of NaN: its columns' sums become NaN
+        bmax = 0;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if ((int)byte_of(vb[d], i) == kBadByte) {
+              if (col_ok) l = NAN;
+              vb[d] &= ~(0xFFu << (8 * i));
+            }
+            bmax = max(bmax, (int)byte_of(vb[d], i));
           }
-          bmax = max(bmax, (int)byte_of(vb[d], i));
-        }
-    }
-    if (__ballot(top > m + 7.f || bmax > E)) {
-      const float m1 = fmaxf(m, column_max(top));
-      const int E1 = max(E, column_max(bmax));
-      const float r = fast_exp2(m - m1);
-      l *= r;
-      const float ro = ldexpf(r, E - E1);
-#pragma unroll
-      for (int i = 0; i < ND; ++i) O[i] *= ro;
-      m = m1;
-      E = E1;
-    }
-    // p = 2^(s - m + 8), and P' = p * 2^(byte - E) in f16 parts.
-    f16v8_t P[2][PP];
-#pragma unroll
-    for (int p = 0; p < 4; ++p)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = fast_exp2(S[p][i] - m + 8.f);
-        l += e;
-        float x = ldexpf(e, (int)byte_of(vb[p], i) - E);
-#pragma unroll
-        for (int k = 0; k < PP; ++k) {
-          const _Float16 h = (_Float16)x;
-          P[p / 2][k][4 * (p & 1) + i] = h;
-          x -= (float)h;
-        }
       }
-    const uint32_t vm[4] = {token_mask(valid, 0), token_mask(valid, 1), token_mask(valid, 2), token_mask(valid, 3)};
-    for (int hh = 0; hh < nhe; hh += HB) {
-      u32x4_t raw[HB][ND];
+      if (__ballot(top > m + 7.f || bmax > E)) {
+        const float m1 = fmaxf(m, column_max(top));
+        const int E1 = max(E, column_max(bmax));
+        const float r = fast_exp2(m - m1);
+        l *= r;
+        const float ro = ldexpf(r, E - E1);
 #pragma unroll
-      for (int j = 0; j < HB; ++j) {
-        const uint8_t* hp = vp + (int64_t)(kh0 + min(hh + j, nhe - 1)) * HD * kTile;
-#pragma unroll
-        for (int i = 0; i < ND; ++i) raw[j][i] = __builtin_nontemporal_load((const u32x4_t*)(hp + i * kTile * kTile));
+        for (int i = 0; i < ND; ++i) O[i] *= ro;
+        m = m1;
+        E = E1;
       }
+      // p = 2^(s - m + 8), and P' = p * 2^(byte - E) in f16 parts.
+      f16v8_t P[2][PP];
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = fast_exp2(S[p][i] - (m - 8.f));
+          l += e;
+          float x = ldexpf(e, (int)byte_of(vb[p], i) - E);
+#pragma unroll
+          for (int k = 0; k < PP; ++k) {
+            const _Float16 h = (_Float16)x;
+            P[p / 2][k][4 * (p & 1) + i] = h;
+            x -= (float)h;
+          }
+        }
       if (tail) {  // a slot past the row may hold anything
+        const uint32_t vm[4] = {token_mask(valid, 0), token_mask(valid, 1), token_mask(valid, 2), token_mask(valid, 3)};
 #pragma unroll
-        for (int j = 0; j < HB; ++j)
+        for (int j = 0; j < NH; ++j)
 #pragma unroll
           for (int i = 0; i < ND; ++i)
 #pragma unroll
-            for (int d = 0; d < 4; ++d) raw[j][i][d] &= vm[d];
+            for (int d = 0; d < 4; ++d) vr[j][i][d] &= vm[d];
       }
 #pragma unroll
-      for (int j = 0; j < HB; ++j) {
-        const bool mine = my == hh + j;
+      for (int j = 0; j < NH; ++j) {
+        const bool mine = NH == 1 || my == j;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           f16v8_t pm[PP];
@@ -729,45 +756,71 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
           for (int k = 0; k < PP; ++k) pm[k] = __builtin_bit_cast(f16v8_t, keep(mine, __builtin_bit_cast(u32x4_t, P[half][k])));
 #pragma unroll
           for (int i = 0; i < ND; ++i) {
-            const f16v8_t vf = codes_f16(raw[j][i][2 * half], raw[j][i][2 * half + 1]);
+            const f16v8_t vf = codes_f16(vr[j][i][2 * half], vr[j][i][2 * half + 1]);
 #pragma unroll
             for (int k = 0; k < PP; ++k) O[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pm[k], O[i], 0, 0, 0);
           }
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      kb = *(const u32x4_t*)(a.c.k + vo1 + byte_off);
+      vb = *(const u32x4_t*)(a.c.v + vo1 + byte_off);
+      vo = vo1;
+      ko1 = tile_offset(a.c, bt, min(4 * (b + 2 * step) + (n >> 2), tlast));
+      vo1 = tile_offset(a.c, bt, min(4 * (b + 2 * step) + g, tlast));
+      __builtin_amdgcn_sched_barrier(0);
+      load_v_block(vo);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
-  // Each wave's normalised output and log2 sum, then the waves' weighted mean.
+  // Each wave's normalised output and log2 sum, then, where several waves share
+  // the columns, their weighted mean.
   l = column_sum(l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (g == 0) lse_sh[wave][n] = l == 0.f ? -INFINITY : m - 8.f + __log2f(l);
+  const float lse = l == 0.f ? -INFINITY : m - 8.f + __log2f(l);
+  const int64_t part = ((int64_t)ri * a.nsplit + split) * a.n_heads + h0;
+  if (a.tw == 1) {
+    if (!col_ok) return;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      float o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = ldexpf(O[i][r] * inv, E - 127);
+      const int d = 16 * i + 4 * g;
+      if (a.nsplit == 1) store_out4(a, (int64_t)row * a.ldo + (int64_t)(h0 + n) * HD + d, o);
+      else *(float4*)(a.part + (part + n) * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+    }
+    if (a.nsplit > 1 && g == 0) a.lse[part + n] = lse;
+    return;
+  }
+  float* lse_sh = o_sh + waves * 16 * kPitch;
+  if (g == 0) lse_sh[wave * 16 + n] = lse;
 #pragma unroll
   for (int i = 0; i < ND; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o_sh[wave][n][16 * i + 4 * g + r] = ldexpf(O[i][r] * inv, E - 127);
+    for (int r = 0; r < 4; ++r) o_sh[(wave * 16 + n) * kPitch + 16 * i + 4 * g + r] = ldexpf(O[i][r] * inv, E - 127);
   __syncthreads();
-  for (int t = threadIdx.x; t < 16 * HD / 4; t += kDecodeWaves * 64) {
+  const int w0 = wave - tpart;
+  for (int t = tpart * 64 + lane; t < ncol * (HD / 4); t += a.tw * 64) {
     const int col = t / (HD / 4), d = t % (HD / 4) * 4;
-    if (col >= ncol) continue;
     float top = -INFINITY;
-    for (int w = 0; w < kDecodeWaves; ++w) top = fmaxf(top, lse_sh[w][col]);
+    for (int w = w0; w < w0 + a.tw; ++w) top = fmaxf(top, lse_sh[w * 16 + col]);
     float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-    for (int w = 0; w < kDecodeWaves; ++w) {
-      const float lw = lse_sh[w][col];
+    for (int w = w0; w < w0 + a.tw; ++w) {
+      const float lw = lse_sh[w * 16 + col];
       if (lw == -INFINITY) continue;
       const float f = fast_exp2(lw - top);
       sum += f;
-      for (int i = 0; i < 4; ++i) o[i] += f * o_sh[w][col][d + i];
+      for (int i = 0; i < 4; ++i) o[i] += f * o_sh[(w * 16 + col) * kPitch + d + i];
     }
     const float norm = sum == 0.f ? 0.f : 1.f / sum;
     for (int i = 0; i < 4; ++i) o[i] *= norm;
     if (a.nsplit == 1) {
       store_out4(a, (int64_t)row * a.ldo + (int64_t)(h0 + col) * HD + d, o);
     } else {
-      const int64_t at = ((int64_t)ri * a.nsplit + split) * a.n_heads + h0 + col;
-      *(float4*)(a.part + at * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
-      if (d == 0) a.lse[at] = sum == 0.f ? -INFINITY : top + __log2f(sum);
+      *(float4*)(a.part + (part + col) * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+      if (d == 0) a.lse[part + col] = sum == 0.f ? -INFINITY : top + __log2f(sum);
     }
   }
 }
@@ -975,12 +1028,13 @@ __global__ __launch_bounds__(kChunkWaves * 64) void kv8_chunk_kernel(const AttnA
 }
 
 // The splits of a row's head joined: the mean of their outputs weighted by
-// their sums.  One thread per 4 dims.  A slot is a decode row or a tile's row.
+// their sums.  A wave per (slot, head), a slot being a decode row or a tile's
+// row: HD / 4 lanes take 4 dims each, the lanes' groups every (256 / HD)-th split.
+template <int HD>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(const AttnArgs a, int64_t slots) {
-  const int HD = a.c.head_dim, q4 = HD / 4;
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int d = (int)(gid % q4) * 4;
-  const int64_t sh = gid / q4;
+  constexpr int L = HD / 4, G = 64 / L;
+  const int lane = threadIdx.x & 63, d = lane % L * 4;
+  const int64_t sh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int head = (int)(sh % a.n_heads);
   const int64_t slot = sh / a.n_heads;
   if (slot >= slots) return;
@@ -994,21 +1048,36 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const AttnArgs a, int64_
     row = a.rows ? a.rows[slot] : slot;
   }
   const int64_t first = slot * a.nsplit * a.n_heads + head;
-  float top = -INFINITY;
-  for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, a.lse[first + (int64_t)s * a.n_heads]);
-  float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  for (int s = 0; s < a.nsplit; ++s) {
+  // Each lane group's own running maximum, its sum and its weighted outputs.
+  float top = -INFINITY, sum = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = lane / L; s < a.nsplit; s += G) {
     const int64_t at = first + (int64_t)s * a.n_heads;
     const float ls = a.lse[at];
     if (ls == -INFINITY) continue;  // nothing was written for it
-    const float f = fast_exp2(ls - top);
-    sum += f;
-    const float4 x = *(const float4*)(a.part + at * HD + d);
-    o[0] += f * x.x; o[1] += f * x.y; o[2] += f * x.z; o[3] += f * x.w;
+    const f32x4_t x = *(const f32x4_t*)(a.part + at * HD + d);
+    const float t1 = fmaxf(top, ls);
+    const float f0 = fast_exp2(top - t1), f1 = fast_exp2(ls - t1);
+    sum = sum * f0 + f1;
+    o = o * f0 + x * f1;
+    top = t1;
   }
+  float all = top;
+#pragma unroll
+  for (int w = L; w < 64; w *= 2) all = fmaxf(all, __shfl_xor(all, w, 64));
+  const float f = top == -INFINITY && sum == 0.f ? 0.f : fast_exp2(top - all);
+  sum *= f;
+  o *= f;
+#pragma unroll
+  for (int w = L; w < 64; w *= 2) {
+    sum += __shfl_xor(sum, w, 64);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], w, 64);
+  }
+  if (lane >= L) return;
   const float norm = sum == 0.f ? 0.f : 1.f / sum;
-  for (int i = 0; i < 4; ++i) o[i] *= norm;
-  store_out4(a, row * a.ldo + (int64_t)head * HD + d, o);
+  const float out[4] = {o[0] * norm, o[1] * norm, o[2] * norm, o[3] * norm};
+  store_out4(a, row * a.ldo + (int64_t)head * HD + d, out);
 }
 
 // ---------------------------------------------------------------------------
@@ -1086,7 +1155,7 @@ int kv8_rows(bool gather, const cbis_kv8_cache* c, int n_rows, int dtype, const 
 // Sizes that both the workspace queries and the launches go by.
 struct Plan {
   int nsplit = 1, split_blocks = 1 << 24;
-  int nh = 1, nhb = 1;   // decode
+  int nh = 1, nhb = 1, tw = 1, waves = 1, groups = 1;  // decode
   int ct = 2, ncg = 1;   // chunk
   int64_t slots = 0;     // rows (or tile rows) of the partials
   size_t bytes = 0;
@@ -1101,19 +1170,18 @@ int64_t table_tokens(const cbis_kv8_attn_desc* d) {
   return std::min<int64_t>(std::max<int64_t>(d->bt_stride, 0), (1 << 30) / d->cache.page_size) * d->cache.page_size;
 }
 
-// `units`: workgroups (or waves) of one split; `want`: how many the GPU takes.
-void plan_split(const cbis_kv8_attn_desc* d, int64_t units, int64_t want, int min_blocks, Plan* p) {
+// 64-token blocks of the longest row, as far as the host knows.
+int64_t longest(const cbis_kv8_attn_desc* d) {
   int64_t tok = table_tokens(d);
   if (d->max_kv_len > 0) tok = std::min<int64_t>(tok, d->max_kv_len);
-  const int64_t blocks = std::max<int64_t>(1, cdiv(tok, kBlk));
-  int64_t per;
-  if (d->split_tokens > 0) {
-    per = cdiv(d->split_tokens, kBlk);
-  } else {
-    const int64_t n = std::max<int64_t>(1, want / std::max<int64_t>(1, units));
-    per = std::max<int64_t>(cdiv(blocks, n), min_blocks);
-  }
-  p->nsplit = (int)std::min<int64_t>(cdiv(blocks, per), 1 << 15);
+  return std::max<int64_t>(1, cdiv(tok, kBlk));
+}
+
+// Splits of `per` blocks, unless the caller names their tokens.
+void set_splits(const cbis_kv8_attn_desc* d, int64_t blocks, int64_t per, Plan* p) {
+  if (d->split_tokens > 0) per = d->split_tokens / kBlk;
+  per = std::max<int64_t>(per, cdiv(blocks, 1 << 15));
+  p->nsplit = (int)cdiv(blocks, per);
   p->split_blocks = (int)per;
   if (p->nsplit > 1) p->bytes = (size_t)p->slots * p->nsplit * d->n_heads * (d->cache.head_dim + 1) * 4;
 }
@@ -1121,14 +1189,33 @@ void plan_split(const cbis_kv8_attn_desc* d, int64_t units, int64_t want, int mi
 Plan plan_decode(const cbis_kv8_attn_desc* d) {
   Plan p;
   const int group = d->n_heads / d->cache.n_kv_heads;
-  if (group >= 16) {
+  if (group > 16) {
     p.nhb = d->cache.n_kv_heads * ((group + 15) / 16);
   } else {
-    p.nh = std::min(16 / group, d->cache.n_kv_heads);
+    // kv heads of a workgroup: as many as make 128 dims, have columns and exist.
+    p.nh = 128 / d->cache.head_dim;
+    while (p.nh > 1 && (p.nh * group > 16 || p.nh / 2 >= d->cache.n_kv_heads)) p.nh /= 2;
     p.nhb = (d->cache.n_kv_heads + p.nh - 1) / p.nh;
   }
   p.slots = std::max(d->n_rows, 0);
-  plan_split(d, p.slots * p.nhb, 512, kDecodeWaves, &p);
+  // The waves that share a row's head block: as many as bring the waves to
+  // 4096, two rounds of what the GPU holds, so that rows of half the longest
+  // one's length still fill it; no more than the blocks. us by waves, MI355X:
+  //   192 rows of 256..4096 x 64 heads of 32 (3072 head blocks)  1: 285  2: 277  4: 278  8: 312
+  //   256 rows of 100 x 64 heads of 32 (4096)                    1: 29   2: 35   4: 49   8: 84
+  //   64 rows of 1000 x 64 heads of 32 (1024)                    1: 48   2: 47   4: 50   8: 62
+  //   61 rows of 500..16384, 32 / 8 heads of 128 (488)           1: 563  2: 319  4: 230  8: 193
+  //   16 rows of 1000 x 64 heads of 32 (256)                     1: 37   2: 23   4: 16   8: 17
+  // Past eight waves the keys are split over workgroups, of at least 16 blocks
+  // (a join costs a launch; 1 row of 16384, 8 kv heads of 128: 4 blocks 35 us, 8
+  // 25, 16 25, 32 29; 16 rows of 32768 x 64 heads: 64 blocks 358, 128 357, 256 345).
+  const int64_t units = std::max<int64_t>(1, p.slots * p.nhb), blocks = longest(d);
+  const int64_t part = d->split_tokens > 0 ? std::min<int64_t>(blocks, d->split_tokens / kBlk) : blocks;
+  while (p.tw < kDecodeWaves && units * p.tw < 4096 && p.tw < part) p.tw *= 2;
+  p.waves = std::max(p.tw, 4);
+  p.groups = (int)cdiv(p.nhb, p.waves / p.tw);
+  const int64_t n = std::max<int64_t>(1, 4096 / (units * kDecodeWaves));
+  set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, n), 16), &p);
   return p;
 }
 
@@ -1138,7 +1225,8 @@ Plan plan_chunk(const cbis_kv8_attn_desc* d, int n_tiles) {
   p.ct = 2;
   p.ncg = (CBIS_PREFILL_TILE_ROWS * group + 16 * p.ct - 1) / (16 * p.ct);
   p.slots = (int64_t)std::max(n_tiles, 0) * CBIS_PREFILL_TILE_ROWS;
-  plan_split(d, (int64_t)std::max(n_tiles, 0) * d->cache.n_kv_heads * p.ncg, 2048, 8, &p);
+  const int64_t units = std::max<int64_t>(1, (int64_t)n_tiles * d->cache.n_kv_heads * p.ncg), blocks = longest(d);
+  set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, 2048 / units)), 8), &p);
   return p;
 }
 
@@ -1192,18 +1280,32 @@ int take_workspace(const cbis_kv8_attn_desc* d, const Plan& p, AttnArgs* a, cons
 }
 
 int merge(const AttnArgs& a, const Plan& p, hipStream_t s, const char* who) {
-  const int64_t threads = p.slots * a.n_heads * (a.c.head_dim / 4);
-  CBIS_REQUIRE(cdiv(threads, 256) < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
-  kv8_merge_kernel<<<(unsigned)cdiv(threads, 256), 256, 0, s>>>(a, p.slots);
+  const int64_t grid = cdiv(p.slots * a.n_heads, 4);
+  CBIS_REQUIRE(grid < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
+  if (a.c.head_dim == 32) kv8_merge_kernel<32><<<(unsigned)grid, 256, 0, s>>>(a, p.slots);
+  else if (a.c.head_dim == 64) kv8_merge_kernel<64><<<(unsigned)grid, 256, 0, s>>>(a, p.slots);
+  else kv8_merge_kernel<128><<<(unsigned)grid, 256, 0, s>>>(a, p.slots);
   return check_launch(who);
 }
 
+template <int HD, int QP, int PP>
+void decode_heads(const AttnArgs& a, const Plan& p, unsigned grid, hipStream_t s) {
+  const int threads = p.waves * 64;
+  const size_t lds = p.tw > 1 ? (size_t)p.waves * 16 * (HD + 5) * sizeof(float) : 0;
+  if constexpr (HD <= 32) {
+    if (p.nh == 4) return kv8_decode_kernel<HD, 4, QP, PP><<<grid, threads, lds, s>>>(a);
+  }
+  if constexpr (HD <= 64) {
+    if (p.nh == 2) return kv8_decode_kernel<HD, 2, QP, PP><<<grid, threads, lds, s>>>(a);
+  }
+  kv8_decode_kernel<HD, 1, QP, PP><<<grid, threads, lds, s>>>(a);
+}
+
 template <int QP, int PP>
-void decode_parts(const AttnArgs& a, unsigned grid, hipStream_t s) {
-  constexpr int T = kDecodeWaves * 64;
-  if (a.c.head_dim == 32) kv8_decode_kernel<32, QP, PP><<<grid, T, 0, s>>>(a);
-  else if (a.c.head_dim == 64) kv8_decode_kernel<64, QP, PP><<<grid, T, 0, s>>>(a);
-  else kv8_decode_kernel<128, QP, PP><<<grid, T, 0, s>>>(a);
+void decode_parts(const AttnArgs& a, const Plan& p, unsigned grid, hipStream_t s) {
+  if (a.c.head_dim == 32) decode_heads<32, QP, PP>(a, p, grid, s);
+  else if (a.c.head_dim == 64) decode_heads<64, QP, PP>(a, p, grid, s);
+  else decode_heads<128, QP, PP>(a, p, grid, s);
 }
 
 template <int QP, int PP>
@@ -1254,17 +1356,17 @@ int cbis_kv8_attention(const cbis_kv8_attn_desc* d, cbis_stream_t stream) {
   a.rows = d->rows;
   a.row_bt = d->row_bt;
   a.row_pos = d->row_pos;
-  a.nh = p.nh;
   a.nhb = p.nhb;
-  const int64_t grid = p.slots * p.nhb * p.nsplit;
+  a.tw = p.tw;
+  const int64_t grid = p.slots * p.groups * p.nsplit;
   CBIS_REQUIRE(grid < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
   hipStream_t s = (hipStream_t)stream;
   if (a.out_bf16) {
-    if (a.q_bf16) decode_parts<1, 1>(a, (unsigned)grid, s);
-    else decode_parts<2, 1>(a, (unsigned)grid, s);
+    if (a.q_bf16) decode_parts<1, 1>(a, p, (unsigned)grid, s);
+    else decode_parts<2, 1>(a, p, (unsigned)grid, s);
   } else {
-    if (a.q_bf16) decode_parts<1, 2>(a, (unsigned)grid, s);
-    else decode_parts<3, 2>(a, (unsigned)grid, s);
+    if (a.q_bf16) decode_parts<1, 2>(a, p, (unsigned)grid, s);
+    else decode_parts<3, 2>(a, p, (unsigned)grid, s);
   }
   rc = check_launch(who);
   return rc || p.nsplit == 1 ? rc : merge(a, p, s, who);
