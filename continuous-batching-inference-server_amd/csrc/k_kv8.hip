@@ -39,7 +39,6 @@ constexpr int kTile = 16;          // tokens of a cache tile
 constexpr int kBlk = 64;           // tokens a wave takes at a time: four tiles
 constexpr int kBadByte = 255;      // scale byte of a slice with a non-finite value
 constexpr int kDecodeWaves = 8;   // of a workgroup, at most
-constexpr int kChunkWaves = 4;
 constexpr float kLowest = -3.3e38f;  // a running maximum before any score
 
 // ---------------------------------------------------------------------------
@@ -53,12 +52,20 @@ struct Pages {
   int64_t tile_bytes;
 };
 
-// Byte offset of tile t of the sequence with block-table row bt.  Page ids are
+// Byte offset of tile t of a sequence whose page there is `page`.  Page ids are
 // clamped to the pool; the offset passes 32 bits in large pools.
-__device__ inline int64_t tile_offset(const Pages& c, const int* __restrict__ bt, int t) {
-  const unsigned page = min((unsigned)bt[t >> c.tshift], (unsigned)(c.num_pages - 1));
-  return (((int64_t)page << c.tshift) + (t & ((1 << c.tshift) - 1))) * c.tile_bytes;
+__device__ inline int64_t tile_offset(const Pages& c, int page, int t) {
+  const unsigned id = min((unsigned)page, (unsigned)(c.num_pages - 1));
+  return (((int64_t)id << c.tshift) + (t & ((1 << c.tshift) - 1))) * c.tile_bytes;
 }
+
+// The wave's number in its workgroup, as a scalar: what derives from it then stays
+// in scalar registers and its branches are branches.
+__device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
+// A barrier that waits for the wave's LDS accesses only: __syncthreads() would
+// also wait for its global loads, which are meant to stay in flight.
+__device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ inline float pow2_of_byte(unsigned b) { return __uint_as_float(b << 23); }
 
@@ -223,7 +230,7 @@ struct RowPlace {
   bool col_ok;
   RowSlots rs;
   __device__ RowPlace(const RowsArgs& a) {
-    wave = threadIdx.x >> 6;
+    wave = wave_id();
     lane = threadIdx.x & 63;
     window = (int64_t)(blockIdx.x / a.parts) * kTile;
     part = (int)(blockIdx.x % a.parts);
@@ -405,7 +412,7 @@ struct AttnArgs {
   int nhb, tw;  // head blocks of a row, waves of a workgroup that share one
   // chunk
   const int* tiles;
-  int n_tiles, ncg;  // column groups of a (tile, kv head)
+  int n_tiles, ncg;  // column groups of a workgroup's kv heads
 };
 
 // 8 consecutive q values of a column as QP bf16 parts.
@@ -561,24 +568,25 @@ __device__ inline u32x4_t keep(bool mine, u32x4_t w) {
 // Bound by HBM while enough bytes are in flight: a block's K and V are 32
 // registers of loads each (NH * HD = 128), the next block's K is loaded as soon
 // as this one's has been multiplied, V likewise, so that one of the two is
-// always on its way.  Page ids are read two blocks ahead, before the loads whose
-// arrival would otherwise have to be awaited with them.
+// always on its way.  Page ids are read two blocks ahead, before loads that are
+// not yet wanted, since loads arrive in order and awaiting one awaits the older
+// ones; they are turned into addresses only where those are used.
 template <int HD, int NH, int QP, int PP>
 __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const AttnArgs a) {
   constexpr int NK = HD / 32, ND = HD / 16;
   constexpr int kPitch = HD + 4;
   extern __shared__ float o_sh[];  // [wave][16][kPitch], then lse_sh [wave][16]; none where tw is 1
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = wave_id(), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   // All rows' last splits first, their first ones at the end, where the short
   // rows (behind the long ones, if the caller sorts them) fill the tail.  With a
   // row's splits side by side the later (often empty) ones would fall on the
   // same XCDs for every row: workgroup b runs on XCD b % 8.
   // The waves are tw token parts of waves / tw head blocks.
   const int waves = blockDim.x >> 6, hpw = waves / a.tw, groups = (a.nhb + hpw - 1) / hpw;
-  int bid = blockIdx.x;
-  const int hb = bid % groups * hpw + wave / a.tw, tpart = wave % a.tw;
-  bid /= groups;
-  const int ri = bid % a.n_rows, split = a.nsplit - 1 - bid / a.n_rows;
+  unsigned bid = blockIdx.x;
+  const int hb = (int)(bid % (unsigned)groups) * hpw + wave / a.tw, tpart = wave % a.tw;
+  bid /= (unsigned)groups;
+  const int ri = (int)(bid % (unsigned)a.n_rows), split = a.nsplit - 1 - (int)(bid / (unsigned)a.n_rows);
   const int row = a.rows ? a.rows[ri] : ri;
   const int kv = min(a.row_pos[row], a.max_tok - 1) + 1;  // keys 0 .. kv - 1, none when <= 0
   const int* bt = a.bt + (a.row_bt ? a.row_bt[row] : row) * a.bt_stride;
@@ -641,12 +649,13 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
   };
 
   if (b0 < b1) {
-    // Tiles of the block the K loads, and of the one the V loads, are at.
-    int64_t ko = tile_offset(a.c, bt, min(4 * b0 + (n >> 2), tlast));
-    int64_t vo = tile_offset(a.c, bt, min(4 * b0 + g, tlast));
-    int64_t ko1 = tile_offset(a.c, bt, min(4 * (b0 + step) + (n >> 2), tlast));
-    int64_t vo1 = tile_offset(a.c, bt, min(4 * (b0 + step) + g, tlast));
-    load_k_block(ko);
+    // Lane's tiles of block b, for K and for V, and the pages they are in.
+    auto k_tile = [&](int b) { return min(4 * b + (n >> 2), tlast); };
+    auto v_tile = [&](int b) { return min(4 * b + g, tlast); };
+    const int kpage0 = bt[k_tile(b0) >> a.c.tshift], vpage0 = bt[v_tile(b0) >> a.c.tshift];
+    int kpage = bt[k_tile(b0 + step) >> a.c.tshift], vpage = bt[v_tile(b0 + step) >> a.c.tshift];
+    int64_t vo = tile_offset(a.c, vpage0, v_tile(b0));
+    load_k_block(tile_offset(a.c, kpage0, k_tile(b0)));
     u32x4_t kb = *(const u32x4_t*)(a.c.k + vo + byte_off);  // tile g's scale bytes of the column's head
     u32x4_t vb = *(const u32x4_t*)(a.c.v + vo + byte_off);
     load_v_block(vo);
@@ -674,7 +683,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      load_k_block(ko1);
+      load_k_block(tile_offset(a.c, kpage, k_tile(b + step)));
       __builtin_amdgcn_sched_barrier(0);
       const int valid = min(max(kv - (b * kBlk + g * kTile), 0), kTile);  // tokens of tile g inside the row
       const bool tail = (b + 1) * kBlk > kv;
@@ -763,11 +772,11 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      kb = *(const u32x4_t*)(a.c.k + vo1 + byte_off);
-      vb = *(const u32x4_t*)(a.c.v + vo1 + byte_off);
-      vo = vo1;
-      ko1 = tile_offset(a.c, bt, min(4 * (b + 2 * step) + (n >> 2), tlast));
-      vo1 = tile_offset(a.c, bt, min(4 * (b + 2 * step) + g, tlast));
+      vo = tile_offset(a.c, vpage, v_tile(b + step));
+      kb = *(const u32x4_t*)(a.c.k + vo + byte_off);
+      vb = *(const u32x4_t*)(a.c.v + vo + byte_off);
+      kpage = bt[k_tile(b + 2 * step) >> a.c.tshift];
+      vpage = bt[v_tile(b + 2 * step) >> a.c.tshift];
       __builtin_amdgcn_sched_barrier(0);
       load_v_block(vo);
       __builtin_amdgcn_sched_barrier(0);
@@ -825,192 +834,328 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
   }
 }
 
-// Chunks.  A wave owns 16 CT columns of one (tile, kv head): column c is row c /
-// group of the tile and query head c % group of the kv head's group.  K and V
-// go from the cache through registers only; the waves of a workgroup are
-// independent.
-template <int HD, int CT, int QP, int PP>
-__global__ __launch_bounds__(kChunkWaves * 64) void kv8_chunk_kernel(const AttnArgs a) {
-  constexpr int NK = HD / 32, ND = HD / 16;
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  int64_t unit = (int64_t)blockIdx.x * kChunkWaves + (threadIdx.x >> 6);
-  const int cg = (int)(unit % a.ncg);
-  unit /= a.ncg;
-  const int kh = (int)(unit % a.c.kv_heads);
-  unit /= a.c.kv_heads;
-  const int split = (int)(unit % a.nsplit);
-  const int64_t tile = unit / a.nsplit;
-  if (tile >= a.n_tiles) return;
+// Chunks.  A workgroup owns (tile, NH kv heads, a group of their columns, split):
+// column c of a kv head is row c / group of the tile and query head c % group of
+// the head's own.  Each wave has 32 columns of one kv head.  A block of 64 tokens
+// of the NH heads (8 KB of K and of V, NH * HD = 128) is converted to bf16 and f16
+// once, by all waves, into LDS in the order in which the products take it; while
+// a block is multiplied the next one's codes are in registers, on their way from
+// the cache.  The scales go in with the conversion: K's exactly, V's as 2^(byte
+// - E + 6), so that the largest code comes to 448 * 64 and what is lost of small
+// slices stays below 2^-40 of it.  The probabilities' sums are one more product,
+// with a V of ones, on the rounded values that the outputs are made of.
+//
+// Bound by the softmax's vector instructions (per wave and block 32 fma, 32 exp2 at
+// a quarter of their rate, 16 conversions, 16 max), which overlap with the other
+// wave's products only in part.
+constexpr int kChunkCols = 32;  // columns of a wave
+
+template <int HD>
+struct ChunkStage {
+  static constexpr int NH = 128 / HD;
+  u32x4_t k[NH][4][HD / 32][64];  // [head][product][k step][lane] 8 bf16
+  u32x4_t v[NH][HD / 16][2][64];  // [head][dims][half][lane] 8 f16
+  int E[NH];                      // the largest V byte so far
+  uint64_t bad[NH];               // tokens whose V slice is NaN
+};
+
+template <int HD, int SW, int QP, int PP>
+__global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
+  constexpr int NK = HD / 32, ND = HD / 16, NH = 128 / HD, W = 8 / SW, WH = W / NH, CT = kChunkCols / 16;
+  constexpr int KP = HD == 32 ? 2 : 1;  // K loads of a staging item (8 bytes each, else 16)
+  extern __shared__ __align__(16) char lds[];
+  ChunkStage<HD>* stage = (ChunkStage<HD>*)lds;
+  _Float16(*factor)[64] = (_Float16(*)[64])(lds + 2 * sizeof(ChunkStage<HD>));  // a wave's own, of the block it stages
+  const int wave = wave_id(), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  unsigned unit = blockIdx.x;
+  const int cg = (int)(unit % (unsigned)a.ncg);
+  unit /= (unsigned)a.ncg;
+  const int hg = (int)(unit % (unsigned)a.nhb);
+  unit /= (unsigned)a.nhb;
+  const int split = (int)(unit % (unsigned)a.nsplit);
+  const int64_t tile = unit / (unsigned)a.nsplit;
   const int row0 = a.tiles[4 * tile], nv = min(a.tiles[4 * tile + 1], CBIS_PREFILL_TILE_ROWS),
             btr = a.tiles[4 * tile + 2], pos0 = a.tiles[4 * tile + 3];
-  const int c0 = cg * 16 * CT, cols = nv * a.group;
-  if (c0 >= cols) return;
+  const int cols = nv * a.group, wg0 = cg * WH * kChunkCols;
+  if (wg0 >= cols) return;
   const int* bt = a.bt + (int64_t)btr * a.bt_stride;
-  const int last_pos = min(pos0 + (min(c0 + 16 * CT, cols) - 1) / a.group, a.max_tok - 1);
+  const int H = a.c.kv_heads, kh0 = hg * NH, kh = kh0 + wave / WH;
+  const int c0 = wg0 + wave % WH * kChunkCols;
+  const bool busy = kh < H && c0 < cols;  // the others stage only
   const int first_pos = pos0 + c0 / a.group;
+  const int last_pos = min(pos0 + (min(c0 + kChunkCols, cols) - 1) / a.group, a.max_tok - 1);
   int pos[CT];
   bf16v8_t q[CT][NK][QP];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int c = c0 + 16 * ct + n, t = c / a.group, head = kh * a.group + c % a.group;
-    const bool ok = c < cols;
+    const bool ok = busy && c < cols;
     pos[ct] = ok ? min(pos0 + t, a.max_tok - 1) : -1;
 #pragma unroll
     for (int s = 0; s < NK; ++s)
       load_q8<QP>(a, (int64_t)(row0 + t) * a.ldq + (int64_t)head * HD + q_dim<HD>(s, g), ok, q[ct][s]);
   }
-  float m[CT], l[CT];
+  float m[CT];
   int E = 0;
-  f32x4_t O[ND][CT];
+  f32x4_t O[ND][CT], l[CT];  // l: every lane of a column holds its sum four times over
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     m[ct] = kLowest;
-    l[ct] = 0.f;
+    l[ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < ND; ++i) O[i][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  const int kv = last_pos + 1;
+  f16v8_t ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (_Float16)1.f;
+  // The workgroup's keys.
+  const int kv = min(pos0 + (min(wg0 + WH * kChunkCols, cols) - 1) / a.group, a.max_tok - 1) + 1;
   const int nblk = kv > 0 ? (kv + kBlk - 1) / kBlk : 0;
   const int b0 = split * a.split_blocks;
   const int b1 = split == a.nsplit - 1 ? nblk : min(nblk, b0 + a.split_blocks);
   const int tlast = (kv - 1) >> 4;
-  const int64_t codes = (int64_t)a.c.kv_heads * HD * kTile;
-  const int64_t head_codes = (int64_t)kh * HD * kTile;
-  for (int b = b0; b < b1; ++b) {
-    const int64_t ko = tile_offset(a.c, bt, min(4 * b + (n >> 2), tlast));
-    const int64_t vo = tile_offset(a.c, bt, min(4 * b + g, tlast));
-    const uint8_t* kp = a.c.k + ko + head_codes + (n & 3) * HD + (HD == 32 ? 8 : 16) * g;
-    const uint8_t* vp = a.c.v + vo + head_codes + n * kTile;
-    const u32x4_t kb = *(const u32x4_t*)(a.c.k + ko + codes + kh * kTile);
-    u32x4_t vb = *(const u32x4_t*)(a.c.v + vo + codes + kh * kTile);
-    KRaw<HD> kraw[4];
+  const int64_t codes = (int64_t)H * HD * kTile;
+
+  // Staging: item f = wave * SW + i of 8 is 64 lanes' 16 bytes of K and of V.
+  auto k_tile = [&](int b) { return min(4 * b + (n >> 2), tlast); };
+  auto v_tile = [&](int b) { return min(4 * b + g, tlast); };
+  int kpage, vpage;  // of the lane's tiles of the block to load, read a block ahead
+  u32x4_t kraw[SW], vraw[SW];
+  // Scale bytes come as the dwords that hold them: taken out of a byte load they
+  // would be awaited where the load is issued.
+  uint32_t kbyte[SW][KP], vbyte = 0;
+  int Es = 0;  // the largest V byte so far of the head whose V the wave stages
+  auto head_index = [](int f) { return HD == 128 ? 0 : HD == 64 ? f >> 2 : f >> 1; };
+  auto head_of = [&](int f) { return min(kh0 + head_index(f), H - 1); };
+  auto load_block = [&](int b) {
+    const int64_t ko = tile_offset(a.c, kpage, k_tile(b)), vo = tile_offset(a.c, vpage, v_tile(b));
+    kpage = bt[k_tile(b + 1) >> a.c.tshift];
+    vpage = bt[v_tile(b + 1) >> a.c.tshift];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int p = 0; p < 4; ++p) kraw[p] = load_k<HD>(kp + 4 * p * HD);
-    u32x4_t vraw[ND];
+    for (int i = 0; i < SW; ++i) {
+      const int f = wave * SW + i, head = head_of(f);
+      const uint8_t* kp = a.c.k + ko + (int64_t)head * HD * kTile + (n & 3) * HD;
+      const uint32_t* kb = (const uint32_t*)(a.c.k + ko + codes + head * kTile);
+      if constexpr (HD == 32) {
 #pragma unroll
-    for (int i = 0; i < ND; ++i) vraw[i] = *(const u32x4_t*)(vp + i * kTile * kTile);
-    f32x4_t S[4][CT];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const float ks = pow2_of_byte((kb[p] >> (8 * (n & 3))) & 0xFFu);  // 255: NaN scores
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) S[p][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < NK; ++s) {
-        const bf16v8_t kf = codes_bf16(kraw[p].w[2 * s], kraw[p].w[2 * s + 1], ks);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-          for (int k = 0; k < QP; ++k)
-            S[p][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[ct][s][k], S[p][ct], 0, 0, 0);
+        for (int j = 0; j < 2; ++j) {
+          const int p = 2 * (f & 1) + j;
+          const u32x2_t w = *(const u32x2_t*)(kp + 4 * p * HD + 8 * g);
+          kraw[i][2 * j] = w[0];
+          kraw[i][2 * j + 1] = w[1];
+          kbyte[i][j] = kb[p];
+        }
+      } else {
+        const int p = HD == 64 ? f & 3 : f >> 1, h = HD == 64 ? 0 : f & 1;
+        kraw[i] = *(const u32x4_t*)(kp + 4 * p * HD + 16 * g + 64 * h);
+        kbyte[i][0] = kb[p];
       }
+      const int dt = HD == 128 ? f : HD == 64 ? f & 3 : f & 1;
+      vraw[i] = *(const u32x4_t*)(a.c.v + vo + (int64_t)head * HD * kTile + (dt * 16 + n) * kTile);
     }
-    const int t0 = b * kBlk + g * kTile;  // first token of the lane's tile
-    if ((b + 1) * kBlk > first_pos + 1) {
+    vbyte = *(const uint32_t*)(a.c.v + vo + codes + head_of(wave * SW) * kTile + (n & 12));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto store_block = [&](int b, ChunkStage<HD>& st) {
+    const int valid = min(max(kv - (b * kBlk + g * kTile), 0), kTile);  // tokens of tile g that may be seen
+    const bool tail = (b + 1) * kBlk > kv;
+    // The V factors: a lane makes token 16 g + n's, and takes tile g's 16.
+    int byte = n < valid ? (int)byte_of(vbyte, n & 3) : 0;
+    const uint64_t bad = __ballot(byte == kBadByte);
+    if (byte == kBadByte) byte = 0;
+    if (__ballot(byte > Es)) {
+      int top = max(byte, Es);
+#pragma unroll
+      for (int x = 1; x < 64; x *= 2) top = max(top, __shfl_xor(top, x, 64));
+      Es = __builtin_amdgcn_readfirstlane(top);
+    }
+    factor[wave][lane] = (_Float16)ldexpf(1.f, byte - Es + 6);
+    if (lane == 0) {  // the waves of a head write the same
+      const int j = head_index(wave * SW);
+      st.E[j] = Es;
+      st.bad[j] = bad;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const f16v8_t f0 = *(const f16v8_t*)&factor[wave][16 * g], f1 = *(const f16v8_t*)&factor[wave][16 * g + 8];
+#pragma unroll
+    for (int i = 0; i < SW; ++i) {
+      const int f = wave * SW + i;
+      if constexpr (HD == 32) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          st.k[head_index(f)][2 * (f & 1) + j][0][lane] = __builtin_bit_cast(
+              u32x4_t, codes_bf16(kraw[i][2 * j], kraw[i][2 * j + 1], pow2_of_byte(byte_of(kbyte[i][j], n & 3))));
+      } else {
+        const int j = head_index(f), p = HD == 64 ? f & 3 : f >> 1, h = HD == 64 ? 0 : f & 1;
+        const float scale = pow2_of_byte(byte_of(kbyte[i][0], n & 3));  // 255: NaN scores
+        st.k[j][p][2 * h][lane] = __builtin_bit_cast(u32x4_t, codes_bf16(kraw[i][0], kraw[i][1], scale));
+        st.k[j][p][2 * h + 1][lane] = __builtin_bit_cast(u32x4_t, codes_bf16(kraw[i][2], kraw[i][3], scale));
+      }
+      const int j = head_index(f), dt = HD == 128 ? f : HD == 64 ? f & 3 : f & 1;
+      u32x4_t w = vraw[i];
+      if (tail) {  // a slot past the last key may hold anything
+#pragma unroll
+        for (int d = 0; d < 4; ++d) w[d] &= token_mask(valid, d);
+      }
+      st.v[j][dt][0][lane] = __builtin_bit_cast(u32x4_t, codes_f16(w[0], w[1]) * f0);
+      st.v[j][dt][1][lane] = __builtin_bit_cast(u32x4_t, codes_f16(w[2], w[3]) * f1);
+    }
+  };
+
+  if (b0 < b1) {
+    kpage = bt[k_tile(b0) >> a.c.tshift];
+    vpage = bt[v_tile(b0) >> a.c.tshift];
+    load_block(b0);
+    store_block(b0, stage[0]);
+    load_block(b0 + 1);
+    lds_barrier();
+  }
+  for (int b = b0; b < b1; ++b) {
+    const ChunkStage<HD>& st = stage[(b - b0) & 1];
+    if (busy && b * kBlk <= last_pos) {
+      const int j = wave / WH;
+      // Operands come from LDS four at a time, the next four before these are
+      // used (left to itself the compiler reads each just ahead of its product).
+      f32x4_t S[4][CT];
 #pragma unroll
       for (int p = 0; p < 4; ++p)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int ct = 0; ct < CT; ++ct) S[p][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      // Operand y is product op_p(y), k step op_s(y): products alternate, so that no
+      // two instructions in a row wait for the same sums.
+      auto op_p = [](int y) { return NK == 1 ? y : y / (2 * NK) * 2 + (y & 1); };
+      auto op_s = [](int y) { return NK == 1 ? 0 : y % (2 * NK) / 2; };
+      bf16v8_t kf[2][4];
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            if (t0 + 4 * p + i > pos[ct]) S[p][ct][i] = -INFINITY;
-    }
-    if ((b + 1) * kBlk > kv) {  // a slot past the last key may hold anything
-      const int valid = min(max(kv - t0, 0), kTile);
+      for (int x = 0; x < 4; ++x) kf[0][x] = __builtin_bit_cast(bf16v8_t, st.k[j][op_p(x)][op_s(x)][lane]);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const uint32_t mask = token_mask(valid, d);
-        vb[d] &= mask;
+      for (int y = 0; y < NK; ++y) {
+        if (y + 1 < NK) {
 #pragma unroll
-        for (int i = 0; i < ND; ++i) vraw[i][d] &= mask;
-      }
-    }
-    int bmax = 0;
+          for (int x = 0; x < 4; ++x)
+            kf[(y + 1) & 1][x] = __builtin_bit_cast(bf16v8_t, st.k[j][op_p(4 * y + 4 + x)][op_s(4 * y + 4 + x)][lane]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
+        for (int k = 0; k < QP; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bmax = max(bmax, (int)byte_of(vb[d], i));
-    if (__ballot(bmax == kBadByte)) {  // a V slice of NaN: the sums of the columns that see it become NaN
-      bmax = 0;
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if ((int)byte_of(vb[d], i) == kBadByte) {
+          for (int x = 0; x < 4; ++x) {
+            const int p = op_p(4 * y + x), s = op_s(4 * y + x);
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct)
-              if (t0 + 4 * d + i <= pos[ct]) l[ct] = NAN;
-            vb[d] &= ~(0xFFu << (8 * i));
+              S[p][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[y & 1][x], q[ct][s][k], S[p][ct], 0, 0, 0);
           }
-          bmax = max(bmax, (int)byte_of(vb[d], i));
-        }
-    }
-    float top[CT];
-    bool grow = bmax > E;
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      top[ct] = -INFINITY;
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top[ct] = fmaxf(top[ct], S[p][ct][i]);
-      top[ct] *= a.qscale;
-      grow |= top[ct] > m[ct] + 7.f;
-    }
-    if (__ballot(grow)) {
-      int E1 = max(E, column_max(bmax));
-      E1 = __builtin_amdgcn_readfirstlane(E1);  // tile g's bytes are the same in all its lanes
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const float m1 = fmaxf(m[ct], column_max(top[ct]));
-        const float r = fast_exp2(m[ct] - m1);
-        l[ct] *= r;
-        const float ro = ldexpf(r, E - E1);
-#pragma unroll
-        for (int i = 0; i < ND; ++i) O[i][ct] *= ro;
-        m[ct] = m1;
+        __builtin_amdgcn_sched_barrier(0);
       }
-      E = E1;
-    }
-    // V as code * 2^(byte - E + 6) in f16 (at most 448 * 64), P as 2^(s - m + 8).
-    f16v8_t vs[2];
+      constexpr int GV = ND < 4 ? ND : 4, NG = ND / GV;  // V operands of a group, groups of a half
+      f16v8_t vf[2][GV];
+      auto load_vf = [&](int y) {
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
+        for (int x = 0; x < GV; ++x)
+          vf[y & 1][x] = __builtin_bit_cast(f16v8_t, st.v[j][y % NG * GV + x][y / NG][lane]);
+      };
+      load_vf(0);
+      const int t0 = b * kBlk + g * kTile;  // first token of the lane's tile
+      if ((b + 1) * kBlk > first_pos + 1) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        vs[d / 2][4 * (d & 1) + i] = (_Float16)ldexpf(1.f, (int)byte_of(vb[d], i) - E + 6);
+        for (int p = 0; p < 4; ++p)
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      f16v8_t P[CT][PP];
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+            for (int ct = 0; ct < CT; ++ct)
+              if (t0 + 4 * p + i > pos[ct]) S[p][ct][i] = -INFINITY;
+      }
+      const uint64_t bad = st.bad[j];
+      if (bad) {  // a column that sees a V slice of NaN becomes NaN
+        const unsigned mine = (unsigned)(bad >> (16 * g));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float e = fast_exp2(S[2 * half + j / 4][ct][j & 3] * a.qscale - (m[ct] - 8.f));
-          l[ct] += e;
-          float x = e;
+        for (int p = 0; p < 4; ++p)
 #pragma unroll
-          for (int k = 0; k < PP; ++k) {
-            const _Float16 h = (_Float16)x;
-            P[ct][k][j] = h;
-            x -= (float)h;
-          }
-        }
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < ND; ++i) {
-        const f16v8_t vf = codes_f16(vraw[i][2 * half], vraw[i][2 * half + 1]) * vs[half];
+            for (int ct = 0; ct < CT; ++ct)
+              if ((mine & (1u << (4 * p + i))) && S[p][ct][i] != -INFINITY) S[p][ct][i] = NAN;
+      }
+      const int E1 = __builtin_amdgcn_readfirstlane(st.E[j]);
+      if (E1 != E) {
+        const float r = ldexpf(1.f, E - E1);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
+          for (int i = 0; i < ND; ++i) O[i][ct] *= r;
+        E = E1;
+      }
+      float top[CT];
+      bool grow = false;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        top[ct] = -INFINITY;
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top[ct] = fmaxf(top[ct], S[p][ct][i]);
+        top[ct] *= a.qscale;
+        grow |= top[ct] > m[ct] + 7.f;
+      }
+      if (__ballot(grow)) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const float m1 = fmaxf(m[ct], column_max(top[ct]));
+          const float r = fast_exp2(m[ct] - m1);
+          l[ct] *= r;
+#pragma unroll
+          for (int i = 0; i < ND; ++i) O[i][ct] *= r;
+          m[ct] = m1;
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        f16v8_t P[CT][PP];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float x = fast_exp2(S[2 * half + h][ct][i] * a.qscale - (m[ct] - 8.f));
+#pragma unroll
+              for (int k = 0; k < PP; ++k) {
+                const _Float16 y = (_Float16)x;
+                P[ct][k][4 * h + i] = y;
+                x -= (float)y;
+              }
+            }
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int k = 0; k < PP; ++k) l[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[ct][k], l[ct], 0, 0, 0);
+#pragma unroll
+        for (int y = half * NG; y < half * NG + NG; ++y) {
+          if (y + 1 < 2 * NG) load_vf(y + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
           for (int k = 0; k < PP; ++k)
-            O[i][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, P[ct][k], O[i][ct], 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < GV; ++x)
+#pragma unroll
+              for (int ct = 0; ct < CT; ++ct)
+                O[y % NG * GV + x][ct] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[y & 1][x], P[ct][k], O[y % NG * GV + x][ct], 0, 0, 0);
+        }
       }
     }
+    if (b + 1 < b1) {
+      store_block(b + 1, stage[(b + 1 - b0) & 1]);
+      load_block(b + 2);  // behind the last block: its last tile again
+      lds_barrier();
+    }
   }
+  if (!busy) return;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int c = c0 + 16 * ct + n, t = c / a.group, head = kh * a.group + c % a.group;
-    const float sum = column_sum(l[ct]);
+    const float sum = l[ct][0];
     if (c >= cols) continue;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int64_t at = ((tile * CBIS_PREFILL_TILE_ROWS + t) * a.nsplit + split) * a.n_heads + head;
@@ -1028,34 +1173,35 @@ __global__ __launch_bounds__(kChunkWaves * 64) void kv8_chunk_kernel(const AttnA
 }
 
 // The splits of a row's head joined: the mean of their outputs weighted by
-// their sums.  A wave per (slot, head), a slot being a decode row or a tile's
-// row: HD / 4 lanes take 4 dims each, the lanes' groups every (256 / HD)-th split.
+// their sums.  HD / 4 lanes hold 4 dims each; `share` such groups of a wave (a
+// power of two) take a (slot, head)'s splits in turn, a slot being a decode row
+// or a tile's row.
 template <int HD>
-__global__ __launch_bounds__(256) void kv8_merge_kernel(const AttnArgs a, int64_t slots) {
-  constexpr int L = HD / 4, G = 64 / L;
-  const int lane = threadIdx.x & 63, d = lane % L * 4;
-  const int64_t sh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void kv8_merge_kernel(const AttnArgs a, int64_t slots, int share) {
+  constexpr int L = HD / 4;
+  const int lane = threadIdx.x & 63, d = lane % L * 4, w = L * share;
+  const int64_t sh = ((int64_t)blockIdx.x * 256 + threadIdx.x) / w;
   const int head = (int)(sh % a.n_heads);
   const int64_t slot = sh / a.n_heads;
-  if (slot >= slots) return;
-  int64_t row;
-  if (a.tiles) {
+  bool ok = slot < slots;
+  int64_t row = 0;
+  if (ok && a.tiles) {
     const int64_t tile = slot / CBIS_PREFILL_TILE_ROWS;
     const int t = (int)(slot % CBIS_PREFILL_TILE_ROWS);
-    if (t >= a.tiles[4 * tile + 1]) return;
+    ok = t < a.tiles[4 * tile + 1];
     row = (int64_t)a.tiles[4 * tile] + t;
-  } else {
+  } else if (ok) {
     row = a.rows ? a.rows[slot] : slot;
   }
   const int64_t first = slot * a.nsplit * a.n_heads + head;
-  // Each lane group's own running maximum, its sum and its weighted outputs.
+  // Each group's own running maximum, its sum and its weighted outputs.
   float top = -INFINITY, sum = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = lane / L; s < a.nsplit; s += G) {
+  for (int s = lane % w / L; ok && s < a.nsplit; s += share) {
     const int64_t at = first + (int64_t)s * a.n_heads;
     const float ls = a.lse[at];
-    if (ls == -INFINITY) continue;  // nothing was written for it
     const f32x4_t x = *(const f32x4_t*)(a.part + at * HD + d);
+    if (ls == -INFINITY) continue;  // an empty split; its outputs may not be there
     const float t1 = fmaxf(top, ls);
     const float f0 = fast_exp2(top - t1), f1 = fast_exp2(ls - t1);
     sum = sum * f0 + f1;
@@ -1063,18 +1209,16 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const AttnArgs a, int64_
     top = t1;
   }
   float all = top;
-#pragma unroll
-  for (int w = L; w < 64; w *= 2) all = fmaxf(all, __shfl_xor(all, w, 64));
-  const float f = top == -INFINITY && sum == 0.f ? 0.f : fast_exp2(top - all);
+  for (int x = L; x < w; x *= 2) all = fmaxf(all, __shfl_xor(all, x, 64));
+  const float f = sum == 0.f ? 0.f : fast_exp2(top - all);
   sum *= f;
   o *= f;
+  for (int x = L; x < w; x *= 2) {
+    sum += __shfl_xor(sum, x, 64);
 #pragma unroll
-  for (int w = L; w < 64; w *= 2) {
-    sum += __shfl_xor(sum, w, 64);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], w, 64);
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
   }
-  if (lane >= L) return;
+  if (!ok || lane % w >= L) return;
   const float norm = sum == 0.f ? 0.f : 1.f / sum;
   const float out[4] = {o[0] * norm, o[1] * norm, o[2] * norm, o[3] * norm};
   store_out4(a, row * a.ldo + (int64_t)head * HD + d, out);
@@ -1156,7 +1300,7 @@ int kv8_rows(bool gather, const cbis_kv8_cache* c, int n_rows, int dtype, const 
 struct Plan {
   int nsplit = 1, split_blocks = 1 << 24;
   int nh = 1, nhb = 1, tw = 1, waves = 1, groups = 1;  // decode
-  int ct = 2, ncg = 1;   // chunk
+  int sw = 1, ncg = 1;   // chunk: staging items of a wave, column groups
   int64_t slots = 0;     // rows (or tile rows) of the partials
   size_t bytes = 0;
 };
@@ -1222,11 +1366,16 @@ Plan plan_decode(const cbis_kv8_attn_desc* d) {
 Plan plan_chunk(const cbis_kv8_attn_desc* d, int n_tiles) {
   Plan p;
   const int group = d->n_heads / d->cache.n_kv_heads;
-  p.ct = 2;
-  p.ncg = (CBIS_PREFILL_TILE_ROWS * group + 16 * p.ct - 1) / (16 * p.ct);
+  // NH kv heads of 128 dims together; as many waves as their columns fill, up to 8.
+  const int NH = 128 / d->cache.head_dim;
+  p.nhb = (d->cache.n_kv_heads + NH - 1) / NH;
+  const int want = (CBIS_PREFILL_TILE_ROWS * group + kChunkCols - 1) / kChunkCols;  // waves of a kv head
+  while (p.sw < 4 / NH && 4 / p.sw >= want * NH) p.sw *= 2;
+  const int wh = 8 / p.sw / NH;
+  p.ncg = (want + wh - 1) / wh;
   p.slots = (int64_t)std::max(n_tiles, 0) * CBIS_PREFILL_TILE_ROWS;
-  const int64_t units = std::max<int64_t>(1, (int64_t)n_tiles * d->cache.n_kv_heads * p.ncg), blocks = longest(d);
-  set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, 2048 / units)), 8), &p);
+  const int64_t units = std::max<int64_t>(1, (int64_t)n_tiles * p.nhb * p.ncg), blocks = longest(d);
+  set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, 256 / units)), 8), &p);
   return p;
 }
 
@@ -1280,11 +1429,13 @@ int take_workspace(const cbis_kv8_attn_desc* d, const Plan& p, AttnArgs* a, cons
 }
 
 int merge(const AttnArgs& a, const Plan& p, hipStream_t s, const char* who) {
-  const int64_t grid = cdiv(p.slots * a.n_heads, 4);
+  int share = 1;  // one group per two splits, as far as the wave has them
+  while (share * 2 <= 256 / a.c.head_dim && share * 2 < p.nsplit) share *= 2;
+  const int64_t grid = cdiv(p.slots * a.n_heads * (a.c.head_dim / 4) * share, 256);
   CBIS_REQUIRE(grid < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
-  if (a.c.head_dim == 32) kv8_merge_kernel<32><<<(unsigned)grid, 256, 0, s>>>(a, p.slots);
-  else if (a.c.head_dim == 64) kv8_merge_kernel<64><<<(unsigned)grid, 256, 0, s>>>(a, p.slots);
-  else kv8_merge_kernel<128><<<(unsigned)grid, 256, 0, s>>>(a, p.slots);
+  if (a.c.head_dim == 32) kv8_merge_kernel<32><<<(unsigned)grid, 256, 0, s>>>(a, p.slots, share);
+  else if (a.c.head_dim == 64) kv8_merge_kernel<64><<<(unsigned)grid, 256, 0, s>>>(a, p.slots, share);
+  else kv8_merge_kernel<128><<<(unsigned)grid, 256, 0, s>>>(a, p.slots, share);
   return check_launch(who);
 }
 
@@ -1308,12 +1459,23 @@ void decode_parts(const AttnArgs& a, const Plan& p, unsigned grid, hipStream_t s
   else decode_heads<128, QP, PP>(a, p, grid, s);
 }
 
+template <int HD, int QP, int PP>
+void chunk_heads(const AttnArgs& a, const Plan& p, unsigned grid, hipStream_t s) {
+  constexpr size_t lds = 2 * sizeof(ChunkStage<HD>) + 8 * 64 * sizeof(_Float16);
+  if constexpr (HD == 128) {
+    if (p.sw == 4) return kv8_chunk_kernel<HD, 4, QP, PP><<<grid, 128, lds, s>>>(a);
+  }
+  if constexpr (HD >= 64) {
+    if (p.sw == 2) return kv8_chunk_kernel<HD, 2, QP, PP><<<grid, 256, lds, s>>>(a);
+  }
+  kv8_chunk_kernel<HD, 1, QP, PP><<<grid, 512, lds, s>>>(a);
+}
+
 template <int QP, int PP>
-void chunk_parts(const AttnArgs& a, unsigned grid, hipStream_t s) {
-  constexpr int T = kChunkWaves * 64;
-  if (a.c.head_dim == 32) kv8_chunk_kernel<32, 2, QP, PP><<<grid, T, 0, s>>>(a);
-  else if (a.c.head_dim == 64) kv8_chunk_kernel<64, 2, QP, PP><<<grid, T, 0, s>>>(a);
-  else kv8_chunk_kernel<128, 2, QP, PP><<<grid, T, 0, s>>>(a);
+void chunk_parts(const AttnArgs& a, const Plan& p, unsigned grid, hipStream_t s) {
+  if (a.c.head_dim == 32) chunk_heads<32, QP, PP>(a, p, grid, s);
+  else if (a.c.head_dim == 64) chunk_heads<64, QP, PP>(a, p, grid, s);
+  else chunk_heads<128, QP, PP>(a, p, grid, s);
 }
 
 }  // namespace
@@ -1365,8 +1527,7 @@ int cbis_kv8_attention(const cbis_kv8_attn_desc* d, cbis_stream_t stream) {
     if (a.q_bf16) decode_parts<1, 1>(a, p, (unsigned)grid, s);
     else decode_parts<2, 1>(a, p, (unsigned)grid, s);
   } else {
-    if (a.q_bf16) decode_parts<1, 2>(a, p, (unsigned)grid, s);
-    else decode_parts<3, 2>(a, p, (unsigned)grid, s);
+    decode_parts<3, 2>(a, p, (unsigned)grid, s);  // bf16 q: its second and third parts are zero
   }
   rc = check_launch(who);
   return rc || p.nsplit == 1 ? rc : merge(a, p, s, who);
@@ -1390,15 +1551,15 @@ int cbis_kv8_chunk_attention(const cbis_kv8_attn_desc* d, int n_tiles, const int
   a.tiles = tiles;
   a.n_tiles = n_tiles;
   a.ncg = p.ncg;
-  const int64_t grid = cdiv((int64_t)n_tiles * p.nsplit * d->cache.n_kv_heads * p.ncg, kChunkWaves);
+  a.nhb = p.nhb;
+  const int64_t grid = (int64_t)n_tiles * p.nsplit * p.nhb * p.ncg;
   CBIS_REQUIRE(grid < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
   hipStream_t s = (hipStream_t)stream;
   if (a.out_bf16) {
-    if (a.q_bf16) chunk_parts<1, 1>(a, (unsigned)grid, s);
-    else chunk_parts<2, 1>(a, (unsigned)grid, s);
+    if (a.q_bf16) chunk_parts<1, 1>(a, p, (unsigned)grid, s);
+    else chunk_parts<2, 1>(a, p, (unsigned)grid, s);
   } else {
-    if (a.q_bf16) chunk_parts<1, 2>(a, (unsigned)grid, s);
-    else chunk_parts<3, 2>(a, (unsigned)grid, s);
+    chunk_parts<3, 2>(a, p, (unsigned)grid, s);
   }
   rc = check_launch(who);
   return rc || p.nsplit == 1 ? rc : merge(a, p, s, who);
