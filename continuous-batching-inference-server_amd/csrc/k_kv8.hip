@@ -412,7 +412,7 @@ struct AttnArgs {
   int nhb, tw;  // head blocks of a row, waves of a workgroup that share one
   // chunk
   const int* tiles;
-  int n_tiles, ncg;  // column groups of a workgroup's kv heads
+  int n_tiles, ncg;  // column groups of a kv head
 };
 
 // 8 consecutive q values of a column as QP bf16 parts.
@@ -834,13 +834,14 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
   }
 }
 
-// Chunks.  A workgroup owns (tile, NH kv heads, a group of their columns, split):
-// column c of a kv head is row c / group of the tile and query head c % group of
-// the head's own.  Each wave has 32 columns of one kv head.  A block of 64 tokens
-// of the NH heads (8 KB of K and of V, NH * HD = 128) is converted to bf16 and f16
-// once, by all waves, into LDS in the order in which the products take it; while
-// a block is multiplied the next one's codes are in registers, on their way from
-// the cache.  The scales go in with the conversion: K's exactly, V's as 2^(byte
+// Chunks at head_dim 64 and 128.  A workgroup owns (tile, kv head, a group of its columns, split): column
+// c is row c / group of the tile and query head c % group of the kv head's own.
+// Each wave has 32 columns and one of KG parts of the keys (KG * HD = 128), whose
+// results are joined at the end (two heads of 64 together instead: 61 us for two
+// chunks of 512 rows after 2048 x 32 heads, two parts of the keys 45: the work
+// comes in smaller pieces).  KG blocks of 64 tokens (8 KB of K and of V) are converted to bf16 and f16 once, by all waves, into LDS
+// in the order in which the products take them; while they are multiplied the
+// next ones' codes are in registers, on their way from the cache.  The scales go in with the conversion: K's exactly, V's as 2^(byte
 // - E + 6), so that the largest code comes to 448 * 64 and what is lost of small
 // slices stays below 2^-40 of it.  The probabilities' sums are one more product,
 // with a V of ones, on the rounded values that the outputs are made of.
@@ -848,21 +849,33 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
 // Bound by the softmax's vector instructions (per wave and block 32 fma, 32 exp2 at
 // a quarter of their rate, 16 conversions, 16 max), which overlap with the other
 // wave's products only in part.
-constexpr int kChunkCols = 32;  // columns of a wave
+constexpr int kChunkCols = 32;  // columns of a wave at head_dim 32
+// The other head dims: 16 where three parts of q of 128 dims would not leave room
+// for the rest (28 / 4 heads of 128, 1024 fp32 rows after 2048: 32 columns spill
+// and take 200 us, 16 101).
+constexpr int chunk_cols(int hd, int qp) { return hd == 128 && qp == 3 ? 16 : kChunkCols; }
 
 template <int HD>
 struct ChunkStage {
-  static constexpr int NH = 128 / HD;
-  u32x4_t k[NH][4][HD / 32][64];  // [head][product][k step][lane] 8 bf16
-  u32x4_t v[NH][HD / 16][2][64];  // [head][dims][half][lane] 8 f16
-  int E[NH];                      // the largest V byte so far
-  uint64_t bad[NH];               // tokens whose V slice is NaN
+  static constexpr int KG = 128 / HD;
+  u32x4_t k[KG][4][HD / 32][64];  // [block][product][k step][lane] 8 bf16
+  u32x4_t v[KG][HD / 16][2][64];  // [block][dims][half][lane] 8 f16
+  int E[KG];                      // the largest V byte so far of the part
+  uint64_t bad[KG];               // tokens whose V slice is NaN
 };
+
+// LDS of a workgroup of the chunk kernel: two stages and the waves' V factors,
+// and at the end, in the same place, the parts' results.
+template <int HD>
+constexpr size_t chunk_lds(int waves) {
+  const size_t stages = 2 * sizeof(ChunkStage<HD>) + waves * 64 * sizeof(_Float16);
+  const size_t join = HD == 128 ? 0 : (size_t)waves * 32 * (HD + 5) * sizeof(float);
+  return stages > join ? stages : join;
+}
 
 template <int HD, int SW, int QP, int PP>
 __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
-  constexpr int NK = HD / 32, ND = HD / 16, NH = 128 / HD, W = 8 / SW, WH = W / NH, CT = kChunkCols / 16;
-  constexpr int KP = HD == 32 ? 2 : 1;  // K loads of a staging item (8 bytes each, else 16)
+  constexpr int NK = HD / 32, ND = HD / 16, KG = 128 / HD, W = 8 / SW, WH = W / KG, COLS = chunk_cols(HD, QP), CT = COLS / 16;
   extern __shared__ __align__(16) char lds[];
   ChunkStage<HD>* stage = (ChunkStage<HD>*)lds;
   _Float16(*factor)[64] = (_Float16(*)[64])(lds + 2 * sizeof(ChunkStage<HD>));  // a wave's own, of the block it stages
@@ -870,20 +883,21 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
   unsigned unit = blockIdx.x;
   const int cg = (int)(unit % (unsigned)a.ncg);
   unit /= (unsigned)a.ncg;
-  const int hg = (int)(unit % (unsigned)a.nhb);
-  unit /= (unsigned)a.nhb;
+  const int kh = (int)(unit % (unsigned)a.c.kv_heads);
+  unit /= (unsigned)a.c.kv_heads;
   const int split = (int)(unit % (unsigned)a.nsplit);
   const int64_t tile = unit / (unsigned)a.nsplit;
+  // Tiles are handed over as cbis_paged_prefill_attention's: row, rows, table row, position.
   const int row0 = a.tiles[4 * tile], nv = min(a.tiles[4 * tile + 1], CBIS_PREFILL_TILE_ROWS),
             btr = a.tiles[4 * tile + 2], pos0 = a.tiles[4 * tile + 3];
-  const int cols = nv * a.group, wg0 = cg * WH * kChunkCols;
+  const int cols = nv * a.group, wg0 = cg * WH * COLS;
   if (wg0 >= cols) return;
   const int* bt = a.bt + (int64_t)btr * a.bt_stride;
-  const int H = a.c.kv_heads, kh0 = hg * NH, kh = kh0 + wave / WH;
-  const int c0 = wg0 + wave % WH * kChunkCols;
-  const bool busy = kh < H && c0 < cols;  // the others stage only
+  const int H = a.c.kv_heads, j = wave / WH;  // j: the wave's part of the keys
+  const int c0 = wg0 + wave % WH * COLS;
+  const bool busy = c0 < cols;  // the others stage only
   const int first_pos = pos0 + c0 / a.group;
-  const int last_pos = min(pos0 + (min(c0 + kChunkCols, cols) - 1) / a.group, a.max_tok - 1);
+  const int last_pos = min(pos0 + (min(c0 + COLS, cols) - 1) / a.group, a.max_tok - 1);
   int pos[CT];
   bf16v8_t q[CT][NK][QP];
 #pragma unroll
@@ -909,24 +923,26 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (_Float16)1.f;
   // The workgroup's keys.
-  const int kv = min(pos0 + (min(wg0 + WH * kChunkCols, cols) - 1) / a.group, a.max_tok - 1) + 1;
+  const int kv = min(pos0 + (min(wg0 + WH * COLS, cols) - 1) / a.group, a.max_tok - 1) + 1;
   const int nblk = kv > 0 ? (kv + kBlk - 1) / kBlk : 0;
   const int b0 = split * a.split_blocks;
   const int b1 = split == a.nsplit - 1 ? nblk : min(nblk, b0 + a.split_blocks);
   const int tlast = (kv - 1) >> 4;
+  const int rounds = (b1 - b0 + KG - 1) / KG;
   const int64_t codes = (int64_t)H * HD * kTile;
+  const int64_t head_codes = (int64_t)kh * HD * kTile, head_bytes = codes + kh * kTile;
 
   // Staging: item f = wave * SW + i of 8 is 64 lanes' 16 bytes of K and of V.
-  auto k_tile = [&](int b) { return min(4 * b + (n >> 2), tlast); };
-  auto v_tile = [&](int b) { return min(4 * b + g, tlast); };
-  int kpage, vpage;  // of the lane's tiles of the block to load, read a block ahead
+  const int js = HD == 128 ? 0 : wave * SW >> 2;  // the part whose blocks the wave stages
+  auto block_of = [&](int r, int part) { return b0 + r * KG + part; };
+  auto k_tile = [&](int r) { return min(4 * block_of(r, js) + (n >> 2), tlast); };
+  auto v_tile = [&](int r) { return min(4 * block_of(r, js) + g, tlast); };
+  int kpage, vpage;  // of the lane's tiles of the block to load, read a round ahead
   u32x4_t kraw[SW], vraw[SW];
   // Scale bytes come as the dwords that hold them: taken out of a byte load they
   // would be awaited where the load is issued.
-  uint32_t kbyte[SW][KP], vbyte = 0;
-  int Es = 0;  // the largest V byte so far of the head whose V the wave stages
-  auto head_index = [](int f) { return HD == 128 ? 0 : HD == 64 ? f >> 2 : f >> 1; };
-  auto head_of = [&](int f) { return min(kh0 + head_index(f), H - 1); };
+  uint32_t kbyte[SW], vbyte = 0;
+  int Es = 0;  // the largest V byte so far of that part
   auto load_block = [&](int b) {
     const int64_t ko = tile_offset(a.c, kpage, k_tile(b)), vo = tile_offset(a.c, vpage, v_tile(b));
     kpage = bt[k_tile(b + 1) >> a.c.tshift];
@@ -934,30 +950,19 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < SW; ++i) {
-      const int f = wave * SW + i, head = head_of(f);
-      const uint8_t* kp = a.c.k + ko + (int64_t)head * HD * kTile + (n & 3) * HD;
-      const uint32_t* kb = (const uint32_t*)(a.c.k + ko + codes + head * kTile);
-      if constexpr (HD == 32) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int p = 2 * (f & 1) + j;
-          const u32x2_t w = *(const u32x2_t*)(kp + 4 * p * HD + 8 * g);
-          kraw[i][2 * j] = w[0];
-          kraw[i][2 * j + 1] = w[1];
-          kbyte[i][j] = kb[p];
-        }
-      } else {
-        const int p = HD == 64 ? f & 3 : f >> 1, h = HD == 64 ? 0 : f & 1;
-        kraw[i] = *(const u32x4_t*)(kp + 4 * p * HD + 16 * g + 64 * h);
-        kbyte[i][0] = kb[p];
-      }
-      const int dt = HD == 128 ? f : HD == 64 ? f & 3 : f & 1;
-      vraw[i] = *(const u32x4_t*)(a.c.v + vo + (int64_t)head * HD * kTile + (dt * 16 + n) * kTile);
+      const int f = wave * SW + i;
+      const uint8_t* kp = a.c.k + ko + head_codes + (n & 3) * HD;
+      const uint32_t* kb = (const uint32_t*)(a.c.k + ko + head_bytes);
+      const int p = HD == 64 ? f & 3 : f >> 1, h = HD == 64 ? 0 : f & 1, dt = HD == 64 ? f & 3 : f;
+      kraw[i] = *(const u32x4_t*)(kp + 4 * p * HD + 16 * g + 64 * h);
+      kbyte[i] = kb[p];
+      vraw[i] = *(const u32x4_t*)(a.c.v + vo + head_codes + (dt * 16 + n) * kTile);
     }
-    vbyte = *(const uint32_t*)(a.c.v + vo + codes + head_of(wave * SW) * kTile + (n & 12));
+    vbyte = *(const uint32_t*)(a.c.v + vo + head_bytes + (n & 12));
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto store_block = [&](int b, ChunkStage<HD>& st) {
+  auto store_block = [&](int r, ChunkStage<HD>& st) {
+    const int b = block_of(r, js);
     const int valid = min(max(kv - (b * kBlk + g * kTile), 0), kTile);  // tokens of tile g that may be seen
     const bool tail = (b + 1) * kBlk > kv;
     // The V factors: a lane makes token 16 g + n's, and takes tile g's 16.
@@ -971,50 +976,41 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
       Es = __builtin_amdgcn_readfirstlane(top);
     }
     factor[wave][lane] = (_Float16)ldexpf(1.f, byte - Es + 6);
-    if (lane == 0) {  // the waves of a head write the same
-      const int j = head_index(wave * SW);
-      st.E[j] = Es;
-      st.bad[j] = bad;
+    if (lane == 0) {  // the waves of a part write the same
+      st.E[js] = Es;
+      st.bad[js] = bad;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const f16v8_t f0 = *(const f16v8_t*)&factor[wave][16 * g], f1 = *(const f16v8_t*)&factor[wave][16 * g + 8];
 #pragma unroll
     for (int i = 0; i < SW; ++i) {
       const int f = wave * SW + i;
-      if constexpr (HD == 32) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          st.k[head_index(f)][2 * (f & 1) + j][0][lane] = __builtin_bit_cast(
-              u32x4_t, codes_bf16(kraw[i][2 * j], kraw[i][2 * j + 1], pow2_of_byte(byte_of(kbyte[i][j], n & 3))));
-      } else {
-        const int j = head_index(f), p = HD == 64 ? f & 3 : f >> 1, h = HD == 64 ? 0 : f & 1;
-        const float scale = pow2_of_byte(byte_of(kbyte[i][0], n & 3));  // 255: NaN scores
-        st.k[j][p][2 * h][lane] = __builtin_bit_cast(u32x4_t, codes_bf16(kraw[i][0], kraw[i][1], scale));
-        st.k[j][p][2 * h + 1][lane] = __builtin_bit_cast(u32x4_t, codes_bf16(kraw[i][2], kraw[i][3], scale));
-      }
-      const int j = head_index(f), dt = HD == 128 ? f : HD == 64 ? f & 3 : f & 1;
+      const int p = HD == 64 ? f & 3 : f >> 1, h = HD == 64 ? 0 : f & 1, dt = HD == 64 ? f & 3 : f;
+      const float scale = pow2_of_byte(byte_of(kbyte[i], n & 3));  // 255: NaN scores
+      st.k[js][p][2 * h][lane] = __builtin_bit_cast(u32x4_t, codes_bf16(kraw[i][0], kraw[i][1], scale));
+      st.k[js][p][2 * h + 1][lane] = __builtin_bit_cast(u32x4_t, codes_bf16(kraw[i][2], kraw[i][3], scale));
       u32x4_t w = vraw[i];
       if (tail) {  // a slot past the last key may hold anything
 #pragma unroll
         for (int d = 0; d < 4; ++d) w[d] &= token_mask(valid, d);
       }
-      st.v[j][dt][0][lane] = __builtin_bit_cast(u32x4_t, codes_f16(w[0], w[1]) * f0);
-      st.v[j][dt][1][lane] = __builtin_bit_cast(u32x4_t, codes_f16(w[2], w[3]) * f1);
+      st.v[js][dt][0][lane] = __builtin_bit_cast(u32x4_t, codes_f16(w[0], w[1]) * f0);
+      st.v[js][dt][1][lane] = __builtin_bit_cast(u32x4_t, codes_f16(w[2], w[3]) * f1);
     }
   };
 
-  if (b0 < b1) {
-    kpage = bt[k_tile(b0) >> a.c.tshift];
-    vpage = bt[v_tile(b0) >> a.c.tshift];
-    load_block(b0);
-    store_block(b0, stage[0]);
-    load_block(b0 + 1);
+  if (rounds > 0) {
+    kpage = bt[k_tile(0) >> a.c.tshift];
+    vpage = bt[v_tile(0) >> a.c.tshift];
+    load_block(0);
+    store_block(0, stage[0]);
+    load_block(1);
     lds_barrier();
   }
-  for (int b = b0; b < b1; ++b) {
-    const ChunkStage<HD>& st = stage[(b - b0) & 1];
-    if (busy && b * kBlk <= last_pos) {
-      const int j = wave / WH;
+  for (int r = 0; r < rounds; ++r) {
+    const ChunkStage<HD>& st = stage[r & 1];
+    const int b = block_of(r, j);
+    if (busy && b < b1 && b * kBlk <= last_pos) {
       // Operands come from LDS four at a time, the next four before these are
       // used (left to itself the compiler reads each just ahead of its product).
       f32x4_t S[4][CT];
@@ -1024,8 +1020,8 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
         for (int ct = 0; ct < CT; ++ct) S[p][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       // Operand y is product op_p(y), k step op_s(y): products alternate, so that no
       // two instructions in a row wait for the same sums.
-      auto op_p = [](int y) { return NK == 1 ? y : y / (2 * NK) * 2 + (y & 1); };
-      auto op_s = [](int y) { return NK == 1 ? 0 : y % (2 * NK) / 2; };
+      auto op_p = [](int y) { return y / (2 * NK) * 2 + (y & 1); };
+      auto op_s = [](int y) { return y % (2 * NK) / 2; };
       bf16v8_t kf[2][4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) kf[0][x] = __builtin_bit_cast(bf16v8_t, st.k[j][op_p(x)][op_s(x)][lane]);
@@ -1048,7 +1044,7 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
           }
         __builtin_amdgcn_sched_barrier(0);
       }
-      constexpr int GV = ND < 4 ? ND : 4, NG = ND / GV;  // V operands of a group, groups of a half
+      constexpr int GV = 4, NG = ND / GV;  // V operands of a group, groups of a half
       f16v8_t vf[2][GV];
       auto load_vf = [&](int y) {
 #pragma unroll
@@ -1145,30 +1141,318 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
         }
       }
     }
-    if (b + 1 < b1) {
-      store_block(b + 1, stage[(b + 1 - b0) & 1]);
-      load_block(b + 2);  // behind the last block: its last tile again
+    if (r + 1 < rounds) {
+      store_block(r + 1, stage[(r + 1) & 1]);
+      load_block(r + 2);  // behind the last block: the last tile again
       lds_barrier();
     }
   }
-  if (!busy) return;
+  // A column's result: normalised outputs and the log2 of its sum.
+  auto finish = [&](int c, int d, const float* o, float lse) {
+    const int t = c / a.group, head = kh * a.group + c % a.group;
+    if (a.nsplit == 1) {
+      store_out4(a, (int64_t)(row0 + t) * a.ldo + (int64_t)head * HD + d, o);
+    } else {
+      const int64_t at = ((tile * CBIS_PREFILL_TILE_ROWS + t) * a.nsplit + split) * a.n_heads + head;
+      *(float4*)(a.part + at * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+      if (d == 0) a.lse[at] = lse;
+    }
+  };
+  constexpr int kPitch = HD + 4, WC = WH * COLS;
+  float* o_sh = (float*)lds;                 // [part][column][kPitch]
+  float* lse_sh = o_sh + KG * WC * kPitch;   // [part][column]
+  if constexpr (KG > 1) __syncthreads();     // the last round's operands have been read
+  if (busy) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int c = c0 + 16 * ct + n;
+      const float sum = l[ct][0], inv = sum == 0.f ? 0.f : 1.f / sum;
+      const float lse = sum == 0.f ? -INFINITY : m[ct] - 8.f + __log2f(sum);
+      if (KG > 1 && g == 0) lse_sh[j * WC + c - wg0] = lse;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        float o[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[x] = ldexpf(O[i][ct][x] * inv, E - 133);
+        const int d = 16 * i + 4 * g;
+        if constexpr (KG > 1) *(float4*)(o_sh + (j * WC + c - wg0) * kPitch + d) = make_float4(o[0], o[1], o[2], o[3]);
+        else if (c < cols) finish(c, d, o, lse);
+      }
+    }
+  }
+  if constexpr (KG > 1) {
+    __syncthreads();
+    for (int t = threadIdx.x; t < min(cols - wg0, WC) * (HD / 4); t += W * 64) {
+      const int c = t / (HD / 4), d = t % (HD / 4) * 4;
+      float top = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < KG; ++x) top = fmaxf(top, lse_sh[x * WC + c]);
+#pragma unroll
+      for (int x = 0; x < KG; ++x) {
+        const float lw = lse_sh[x * WC + c];
+        if (lw == -INFINITY) continue;
+        const float f = fast_exp2(lw - top);
+        const float4 y = *(const float4*)(o_sh + (x * WC + c) * kPitch + d);
+        sum += f;
+        o[0] += f * y.x; o[1] += f * y.y; o[2] += f * y.z; o[3] += f * y.w;
+      }
+      const float norm = sum == 0.f ? 0.f : 1.f / sum;
+      for (int i = 0; i < 4; ++i) o[i] *= norm;
+      finish(wg0 + c, d, o, sum == 0.f ? -INFINITY : top + __log2f(sum));
+    }
+  }
+}
+
+// Chunks at head_dim 32, where K and V are cheap to convert and the softmax is
+// everything: a wave has 32 columns of a kv head and every tw-th block of 64
+// tokens, straight from the cache through registers like the single rows'
+// kernel, so that waves run apart and fill each other's gaps.
+template <int QP, int PP>
+__global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const AttnArgs a) {
+  constexpr int HD = 32, ND = 2, CT = kChunkCols / 16, kPitch = HD + 4;
+  // Per wave 64 V factors of the block at hand; at the end the parts' results.
+  extern __shared__ __align__(16) char lds[];
+  const int wave = wave_id(), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int waves = blockDim.x >> 6, upw = waves / a.tw, tpart = wave % a.tw;  // upw: units of a workgroup
+  unsigned unit = blockIdx.x * (unsigned)upw + wave / a.tw;
+  const int cg = (int)(unit % (unsigned)a.ncg);
+  unit /= (unsigned)a.ncg;
+  const int kh = (int)(unit % (unsigned)a.c.kv_heads);
+  unit /= (unsigned)a.c.kv_heads;
+  const int split = (int)(unit % (unsigned)a.nsplit);
+  const int tile = (int)(unit / (unsigned)a.nsplit);
+  const bool in = tile < a.n_tiles;
+  const int4 td = in ? *(const int4*)(a.tiles + 4 * (int64_t)tile) : make_int4(0, 0, 0, 0);
+  const int row0 = td.x, nv = min(td.y, CBIS_PREFILL_TILE_ROWS), pos0 = td.w;
+  const int c0 = cg * kChunkCols, cols = nv * a.group;
+  const bool busy = in && c0 < cols;
+  const int* bt = a.bt + (int64_t)td.z * a.bt_stride;
+  const int first_pos = pos0 + c0 / a.group;
+  const int last_pos = min(pos0 + (min(c0 + kChunkCols, cols) - 1) / a.group, a.max_tok - 1);
+  int pos[CT];
+  bf16v8_t q[CT][QP];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int c = c0 + 16 * ct + n, t = c / a.group, head = kh * a.group + c % a.group;
-    const float sum = l[ct][0];
-    if (c >= cols) continue;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int64_t at = ((tile * CBIS_PREFILL_TILE_ROWS + t) * a.nsplit + split) * a.n_heads + head;
+    const bool ok = busy && c < cols;
+    pos[ct] = ok ? min(pos0 + t, a.max_tok - 1) : -1;
+    load_q8<QP>(a, (int64_t)(row0 + t) * a.ldq + (int64_t)head * HD + q_dim<HD>(0, g), ok, q[ct]);
+  }
+  float m[CT];
+  int E = 0;
+  f32x4_t O[ND][CT], l[CT];  // l: every lane of a column holds its sum four times over
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = kLowest;
+    l[ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < ND; ++i) O[i][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  f16v8_t ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (_Float16)1.f;
+
+  const int kv = last_pos + 1;
+  const int nblk = busy && kv > 0 ? (kv + kBlk - 1) / kBlk : 0;
+  const int b0 = split * a.split_blocks + tpart;
+  const int b1 = split == a.nsplit - 1 ? nblk : min(nblk, (split + 1) * a.split_blocks);
+  const int tlast = (kv - 1) >> 4;
+  const int64_t codes = (int64_t)a.c.kv_heads * HD * kTile;
+  const int64_t k_off = (int64_t)kh * HD * kTile + (n & 3) * HD + 8 * g, v_off = (int64_t)kh * HD * kTile + n * kTile;
+  const int64_t byte_off = codes + kh * kTile;
+  _Float16* factor = (_Float16*)lds + wave * 64;
+
+  if (b0 < b1) {
+    auto k_tile = [&](int b) { return min(4 * b + (n >> 2), tlast); };
+    auto v_tile = [&](int b) { return min(4 * b + g, tlast); };
+    KRaw<HD> kr[4];
+    u32x4_t vr[ND], kb;
+    uint32_t vbyte;
+    auto load_k_block = [&](int64_t at) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) kr[p] = load_k<HD>(a.c.k + at + k_off + 4 * p * HD);
+      kb = *(const u32x4_t*)(a.c.k + at + byte_off);
+    };
+    auto load_v_block = [&](int64_t at) {
+      vbyte = *(const uint32_t*)(a.c.v + at + byte_off + (n & 12));
+#pragma unroll
+      for (int i = 0; i < ND; ++i) vr[i] = *(const u32x4_t*)(a.c.v + at + v_off + i * kTile * kTile);
+    };
+    const int kpage0 = bt[k_tile(b0) >> a.c.tshift], vpage0 = bt[v_tile(b0) >> a.c.tshift];
+    int kpage = bt[k_tile(b0 + a.tw) >> a.c.tshift], vpage = bt[v_tile(b0 + a.tw) >> a.c.tshift];
+    load_k_block(tile_offset(a.c, kpage0, k_tile(b0)));
+    load_v_block(tile_offset(a.c, vpage0, v_tile(b0)));
+    for (int b = b0; b < b1; b += a.tw) {
+      f32x4_t S[4][CT];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const float ks = pow2_of_byte(byte_of(kb[p], n & 3));  // 255: NaN scores
+        const bf16v8_t kf = codes_bf16(kr[p].w[0], kr[p].w[1], ks);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          S[p][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < QP; ++k)
+            S[p][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[ct][k], S[p][ct], 0, 0, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_k_block(tile_offset(a.c, kpage, k_tile(b + a.tw)));
+      __builtin_amdgcn_sched_barrier(0);
+      const int t0 = b * kBlk + g * kTile;  // first token of the lane's tile
+      if ((b + 1) * kBlk > first_pos + 1) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+              if (t0 + 4 * p + i > pos[ct]) S[p][ct][i] = -INFINITY;
+      }
+      // V's factors: a lane makes token 16 g + n's, and takes tile g's 16.
+      const int valid = min(max(kv - t0, 0), kTile);  // tokens of tile g that may be seen
+      int byte = n < valid ? (int)byte_of(vbyte, n & 3) : 0;
+      const uint64_t bad = __ballot(byte == kBadByte);
+      if (bad) {  // a column that sees a V slice of NaN becomes NaN
+        if (byte == kBadByte) byte = 0;
+        const unsigned mine = (unsigned)(bad >> (16 * g));
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+              if ((mine & (1u << (4 * p + i))) && S[p][ct][i] != -INFINITY) S[p][ct][i] = NAN;
+      }
+      if (__ballot(byte > E)) {
+        int E1 = max(byte, E);
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) E1 = max(E1, __shfl_xor(E1, x, 64));
+        E1 = __builtin_amdgcn_readfirstlane(E1);
+        const float r = ldexpf(1.f, E - E1);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int i = 0; i < ND; ++i) O[i][ct] *= r;
+        E = E1;
+      }
+      factor[lane] = (_Float16)ldexpf(1.f, byte - E + 6);
+      float top[CT];
+      bool grow = false;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        top[ct] = -INFINITY;
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top[ct] = fmaxf(top[ct], S[p][ct][i]);
+        top[ct] *= a.qscale;
+        grow |= top[ct] > m[ct] + 7.f;
+      }
+      if (__ballot(grow)) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const float m1 = fmaxf(m[ct], column_max(top[ct]));
+          const float r = fast_exp2(m[ct] - m1);
+          l[ct] *= r;
+#pragma unroll
+          for (int i = 0; i < ND; ++i) O[i][ct] *= r;
+          m[ct] = m1;
+        }
+      }
+      if ((b + 1) * kBlk > kv) {  // a slot past the last key may hold anything
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const uint32_t mask = token_mask(valid, d);
+#pragma unroll
+          for (int i = 0; i < ND; ++i) vr[i][d] &= mask;
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const f16v8_t f = *(const f16v8_t*)(factor + 16 * g + 8 * half);
+        f16v8_t P[CT][PP];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float x = fast_exp2(S[2 * half + i / 4][ct][i & 3] * a.qscale - (m[ct] - 8.f));
+#pragma unroll
+            for (int k = 0; k < PP; ++k) {
+              const _Float16 y = (_Float16)x;
+              P[ct][k][i] = y;
+              x -= (float)y;
+            }
+          }
+#pragma unroll
+        for (int k = 0; k < PP; ++k)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            l[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[ct][k], l[ct], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+              O[i][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(vr[i][2 * half], vr[i][2 * half + 1]) * f,
+                                                                P[ct][k], O[i][ct], 0, 0, 0);
+          }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const int64_t vo = tile_offset(a.c, vpage, v_tile(b + a.tw));
+      kpage = bt[k_tile(b + 2 * a.tw) >> a.c.tshift];
+      vpage = bt[v_tile(b + 2 * a.tw) >> a.c.tshift];
+      __builtin_amdgcn_sched_barrier(0);
+      load_v_block(vo);  // behind the last block: the last tile again
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  auto finish = [&](int c, int d, const float* o, float lse) {
+    const int t = c / a.group, head = kh * a.group + c % a.group;
+    if (a.nsplit == 1) {
+      store_out4(a, (int64_t)(row0 + t) * a.ldo + (int64_t)head * HD + d, o);
+    } else {
+      const int64_t at = (((int64_t)tile * CBIS_PREFILL_TILE_ROWS + t) * a.nsplit + split) * a.n_heads + head;
+      *(float4*)(a.part + at * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+      if (d == 0) a.lse[at] = lse;
+    }
+  };
+  float* o_sh = (float*)lds;  // [wave][column][kPitch]
+  float* lse_sh = o_sh + waves * kChunkCols * kPitch;
+  if (a.tw > 1) __syncthreads();
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = c0 + 16 * ct + n;
+    const float sum = l[ct][0], inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float lse = sum == 0.f ? -INFINITY : m[ct] - 8.f + __log2f(sum);
+    if (a.tw > 1 && g == 0) lse_sh[wave * kChunkCols + 16 * ct + n] = lse;
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
       float o[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = ldexpf(O[i][ct][r] * inv, E - 133);
+      for (int x = 0; x < 4; ++x) o[x] = ldexpf(O[i][ct][x] * inv, E - 133);
       const int d = 16 * i + 4 * g;
-      if (a.nsplit == 1) store_out4(a, (int64_t)(row0 + t) * a.ldo + (int64_t)head * HD + d, o);
-      else *(float4*)(a.part + at * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+      if (a.tw > 1) *(float4*)(o_sh + (wave * kChunkCols + 16 * ct + n) * kPitch + d) = make_float4(o[0], o[1], o[2], o[3]);
+      else if (busy && c < cols) finish(c, d, o, lse);
     }
-    if (a.nsplit > 1 && g == 0) a.lse[at] = sum == 0.f ? -INFINITY : m[ct] - 8.f + __log2f(sum);
+  }
+  if (a.tw == 1) return;
+  __syncthreads();
+  if (!busy) return;
+  for (int t = tpart * 64 + lane; t < min(cols - c0, kChunkCols) * (HD / 4); t += a.tw * 64) {
+    const int c = t / (HD / 4), d = t % (HD / 4) * 4, w0 = wave - tpart;
+    float top = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int x = w0; x < w0 + a.tw; ++x) top = fmaxf(top, lse_sh[x * kChunkCols + c]);
+    for (int x = w0; x < w0 + a.tw; ++x) {
+      const float lw = lse_sh[x * kChunkCols + c];
+      if (lw == -INFINITY) continue;
+      const float f = fast_exp2(lw - top);
+      const float4 y = *(const float4*)(o_sh + (x * kChunkCols + c) * kPitch + d);
+      sum += f;
+      o[0] += f * y.x; o[1] += f * y.y; o[2] += f * y.z; o[3] += f * y.w;
+    }
+    const float norm = sum == 0.f ? 0.f : 1.f / sum;
+    for (int i = 0; i < 4; ++i) o[i] *= norm;
+    finish(c0 + c, d, o, sum == 0.f ? -INFINITY : top + __log2f(sum));
   }
 }
 
@@ -1366,16 +1650,34 @@ Plan plan_decode(const cbis_kv8_attn_desc* d) {
 Plan plan_chunk(const cbis_kv8_attn_desc* d, int n_tiles) {
   Plan p;
   const int group = d->n_heads / d->cache.n_kv_heads;
-  // NH kv heads of 128 dims together; as many waves as their columns fill, up to 8.
-  const int NH = 128 / d->cache.head_dim;
-  p.nhb = (d->cache.n_kv_heads + NH - 1) / NH;
-  const int want = (CBIS_PREFILL_TILE_ROWS * group + kChunkCols - 1) / kChunkCols;  // waves of a kv head
-  while (p.sw < 4 / NH && 4 / p.sw >= want * NH) p.sw *= 2;
-  const int wh = 8 / p.sw / NH;
-  p.ncg = (want + wh - 1) / wh;
   p.slots = (int64_t)std::max(n_tiles, 0) * CBIS_PREFILL_TILE_ROWS;
-  const int64_t units = std::max<int64_t>(1, (int64_t)n_tiles * p.nhb * p.ncg), blocks = longest(d);
-  set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, 256 / units)), 8), &p);
+  const int64_t blocks = longest(d);
+  if (d->cache.head_dim == 32) {
+    p.ncg = (CBIS_PREFILL_TILE_ROWS * group + kChunkCols - 1) / kChunkCols;
+    const int64_t units = std::max<int64_t>(1, (int64_t)n_tiles * d->cache.n_kv_heads * p.ncg);
+    const int64_t part = d->split_tokens > 0 ? std::min<int64_t>(blocks, d->split_tokens / kBlk) : blocks;
+    // Waves that share the keys of 32 columns: as many as bring the waves to 2048,
+    // two to a SIMD.  us by that goal, 64 heads of 32, MI355X:
+    //   two chunks of 512, 0 and 512 cached      1: 23.7  2048: 23.5  4096: 23.2  8192: 27.9
+    //   512 rows after 16384                     1: 224   2048: 192   4096: 201   8192: 220
+    //   512 fresh rows                           1: 12.5  2048: 10.8  4096: 13.8  8192: 21.6
+    //   16 rows after 32000                      1: 118   2048: 61    4096: 61    8192: 61
+    while (p.tw < kDecodeWaves && units * p.tw < 2048 && p.tw < part) p.tw *= 2;
+    p.waves = std::max(p.tw, 4);
+    set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, 4096 / (units * kDecodeWaves))), 16), &p);
+    return p;
+  }
+  // As many waves as a kv head's columns fill, times the parts of the keys, up to 8.
+  const int KG = 128 / d->cache.head_dim;
+  const int cols = chunk_cols(d->cache.head_dim, d->out_dtype == CBIS_F32 ? 3 : 1);
+  const int want = (CBIS_PREFILL_TILE_ROWS * group + cols - 1) / cols;
+  while (p.sw < 4 / KG && 4 / p.sw >= want * KG) p.sw *= 2;
+  const int wh = 8 / p.sw / KG;
+  p.ncg = (want + wh - 1) / wh;
+  const int64_t units = std::max<int64_t>(1, (int64_t)n_tiles * d->cache.n_kv_heads * p.ncg);
+  // Splits for one workgroup per CU (512 rows after 16384, 32 / 8 heads of 128: 4
+  // splits 174 us, 8 175 and another 9 us of joining).
+  set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, 256 / units)), 8 * KG), &p);
   return p;
 }
 
@@ -1461,7 +1763,7 @@ void decode_parts(const AttnArgs& a, const Plan& p, unsigned grid, hipStream_t s
 
 template <int HD, int QP, int PP>
 void chunk_heads(const AttnArgs& a, const Plan& p, unsigned grid, hipStream_t s) {
-  constexpr size_t lds = 2 * sizeof(ChunkStage<HD>) + 8 * 64 * sizeof(_Float16);
+  const size_t lds = chunk_lds<HD>(8 / p.sw);
   if constexpr (HD == 128) {
     if (p.sw == 4) return kv8_chunk_kernel<HD, 4, QP, PP><<<grid, 128, lds, s>>>(a);
   }
@@ -1473,9 +1775,14 @@ void chunk_heads(const AttnArgs& a, const Plan& p, unsigned grid, hipStream_t s)
 
 template <int QP, int PP>
 void chunk_parts(const AttnArgs& a, const Plan& p, unsigned grid, hipStream_t s) {
-  if (a.c.head_dim == 32) chunk_heads<32, QP, PP>(a, p, grid, s);
-  else if (a.c.head_dim == 64) chunk_heads<64, QP, PP>(a, p, grid, s);
-  else chunk_heads<128, QP, PP>(a, p, grid, s);
+  if (a.c.head_dim == 32) {
+    const size_t join = p.tw > 1 ? (size_t)p.waves * kChunkCols * (32 + 5) * sizeof(float) : 0;
+    kv8_chunk32_kernel<QP, PP><<<grid, p.waves * 64, std::max(join, (size_t)p.waves * 64 * sizeof(_Float16)), s>>>(a);
+  } else if (a.c.head_dim == 64) {
+    chunk_heads<64, QP, PP>(a, p, grid, s);
+  } else {
+    chunk_heads<128, QP, PP>(a, p, grid, s);
+  }
 }
 
 }  // namespace
@@ -1551,8 +1858,9 @@ int cbis_kv8_chunk_attention(const cbis_kv8_attn_desc* d, int n_tiles, const int
   a.tiles = tiles;
   a.n_tiles = n_tiles;
   a.ncg = p.ncg;
-  a.nhb = p.nhb;
-  const int64_t grid = (int64_t)n_tiles * p.nsplit * p.nhb * p.ncg;
+  a.tw = p.tw;
+  const int64_t units = (int64_t)n_tiles * p.nsplit * d->cache.n_kv_heads * p.ncg;
+  const int64_t grid = d->cache.head_dim == 32 ? cdiv(units, p.waves / p.tw) : units;
   CBIS_REQUIRE(grid < (1LL << 31), CBIS_ERR_UNSUPPORTED, "%s: grid too large", who);
   hipStream_t s = (hipStream_t)stream;
   if (a.out_bf16) {
