@@ -16,6 +16,14 @@ size_t dtype_size(int dtype) {
   }
 }
 
+size_t kv_page_bytes(int page_size, int n_heads, int head_dim, int kv_dtype) {
+  if (kv_dtype != CBIS_FP8E4M3) return (size_t)page_size * n_heads * head_dim * dtype_size(kv_dtype);
+  const size_t bytes = cbis_kv8_page_bytes(n_heads, head_dim, page_size);
+  if (bytes == 0)
+    throw std::invalid_argument("fp8 K/V pages need head_dim 32, 64 or 128 and a page size that is a power of two >= 16");
+  return bytes;
+}
+
 void hip_check(hipError_t e, const char* what) {
   if (e != hipSuccess) throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
 }
@@ -32,7 +40,9 @@ void ModelConfig::validate() const {
   if (max_seq % page_size != 0) throw std::invalid_argument("ModelConfig: max_seq must be page-aligned");
   if (weight_dtype != CBIS_F32 && weight_dtype != CBIS_BF16 && weight_dtype != CBIS_FP8E4M3)
     throw std::invalid_argument("ModelConfig: weight dtype");
-  if (kv_dtype != CBIS_F32 && kv_dtype != CBIS_BF16) throw std::invalid_argument("ModelConfig: kv dtype");
+  if (kv_dtype != CBIS_F32 && kv_dtype != CBIS_BF16 && kv_dtype != CBIS_FP8E4M3)
+    throw std::invalid_argument("ModelConfig: kv dtype");
+  (void)kv_page_bytes(page_size, n_heads, head_dim, kv_dtype);  // throws for a geometry the dtype has no pages for
 }
 
 PagedKVCache::PagedKVCache(int num_layers, int max_pages, int page_size, int n_heads, int head_dim, int kv_dtype,
@@ -46,7 +56,7 @@ PagedKVCache::PagedKVCache(int num_layers, int max_pages, int page_size, int n_h
       pages_per_seq_(pages_per_seq) {
   if (num_layers <= 0 || max_pages <= 0 || page_size <= 0 || n_heads <= 0 || head_dim <= 0 || pages_per_seq <= 0)
     throw std::invalid_argument("PagedKVCache: sizes must be positive");
-  layer_bytes_ = (size_t)max_pages * page_size * n_heads * head_dim * dtype_size(kv_dtype);
+  layer_bytes_ = (size_t)max_pages * kv_page_bytes(page_size, n_heads, head_dim, kv_dtype);
   if (alloc_device) {
     const size_t total = layer_bytes_ * 2 * (size_t)num_layers;
     hip_check(hipMalloc((void**)&base_, total), "PagedKVCache: hipMalloc");
@@ -113,9 +123,49 @@ void* PagedKVCache::v_base(int layer) const {
 
 void PagedKVCache::fill_normal(uint64_t seed, float std, hipStream_t s) {
   if (!base_) throw std::logic_error("PagedKVCache: created without device pools");
+  if (kv_dtype_ == CBIS_FP8E4M3) return fill_normal_kv8(seed, std, s);
   const int64_t n = (int64_t)(layer_bytes_ * 2 * (size_t)num_layers_ / dtype_size(kv_dtype_));
   cbis_check(cbis_fill_normal_fast(base_, kv_dtype_, n, seed, std, s), "PagedKVCache::fill_normal");
   hip_check(hipStreamSynchronize(s), "PagedKVCache::fill_normal sync");
+}
+
+cbis_kv8_cache PagedKVCache::kv8_view(int layer) const {
+  if (kv_dtype_ != CBIS_FP8E4M3) throw std::logic_error("PagedKVCache::kv8_view: not an fp8 cache");
+  return {n_heads_, head_dim_, page_size_, max_pages_, k_base(layer), v_base(layer)};
+}
+
+// fp32 normals, some pages' rows at a time, quantised into their slots.
+void PagedKVCache::fill_normal_kv8(uint64_t seed, float std, hipStream_t s) {
+  const int64_t width = (int64_t)n_heads_ * head_dim_;
+  const int pages = std::min(max_pages_, std::max(1, 4096 / page_size_)), rows = pages * page_size_;
+  std::vector<int> slots(2 * (size_t)rows);  // pages, then offsets
+  struct Buffers {
+    float* x = nullptr;
+    int* slots = nullptr;
+    ~Buffers() {
+      (void)hipFree(x);
+      (void)hipFree(slots);
+    }
+  } d;
+  hip_check(hipMalloc((void**)&d.x, 2 * rows * width * 4), "PagedKVCache::fill_normal: hipMalloc");
+  hip_check(hipMalloc((void**)&d.slots, slots.size() * 4), "PagedKVCache::fill_normal: hipMalloc");
+  for (int first = 0; first < max_pages_; first += pages) {
+    for (int i = 0; i < rows; ++i) {
+      slots[i] = first + i / page_size_;  // past the pool: the row is skipped
+      slots[rows + i] = i % page_size_;
+    }
+    hip_check(hipMemcpyAsync(d.slots, slots.data(), slots.size() * 4, hipMemcpyHostToDevice, s),
+              "PagedKVCache::fill_normal: H2D");
+    hip_check(hipStreamSynchronize(s), "PagedKVCache::fill_normal sync");
+    for (int l = 0; l < num_layers_; ++l) {
+      cbis_check(cbis_fill_normal_fast(d.x, CBIS_F32, 2 * rows * width, seed + (uint64_t)first * num_layers_ + l, std, s),
+                 "PagedKVCache::fill_normal");
+      const cbis_kv8_cache c = kv8_view(l);
+      cbis_check(cbis_kv8_scatter(&c, rows, CBIS_F32, d.x, width, d.x + rows * width, width, d.slots, d.slots + rows, s),
+                 "PagedKVCache::fill_normal");
+    }
+    hip_check(hipStreamSynchronize(s), "PagedKVCache::fill_normal sync");
+  }
 }
 
 }  // namespace cbis

@@ -41,6 +41,8 @@ struct ModelConfig {
 };
 
 size_t dtype_size(int dtype);
+// Bytes of one page of a K or V pool (fp8: with its scale bytes).
+size_t kv_page_bytes(int page_size, int n_heads, int head_dim, int kv_dtype);
 void hip_check(hipError_t e, const char* what);
 void cbis_check(int rc, const char* what);
 
@@ -49,7 +51,8 @@ void cbis_check(int rc, const char* what);
 // exactly (free list [P-1 .. 0] so pop_back hands out 0, 1, 2, ...; pages of
 // a freed sequence are pushed back in logical order; sequence ids are a
 // monotonic counter).  Device pools: one allocation holding, per layer, a K
-// pool then a V pool, each [max_pages][page_size][n_heads][head_dim].
+// pool then a V pool, each [max_pages][page_size][n_heads][head_dim], or pages
+// of the 8-bit format of cbis_kv8_cache (kv_dtype fp8).
 // ---------------------------------------------------------------------------
 class PagedKVCache {
  public:
@@ -79,8 +82,11 @@ class PagedKVCache {
   size_t pool_bytes() const { return layer_bytes_; }
   bool has_device() const { return base_ != nullptr; }
   void fill_normal(uint64_t seed, float std, hipStream_t s);
+  // A layer's pools as the 8-bit calls take them (kv_dtype fp8 only).
+  cbis_kv8_cache kv8_view(int layer) const;
 
  private:
+  void fill_normal_kv8(uint64_t seed, float std, hipStream_t s);
   int num_layers_, max_pages_, page_size_, n_heads_, head_dim_, kv_dtype_, pages_per_seq_;
   size_t layer_bytes_ = 0;
   uint8_t* base_ = nullptr;
@@ -249,7 +255,7 @@ class TransformerRunner {
   // activations
   float* d_x_ = nullptr;
   void* d_xn_ = nullptr;
-  float* d_q_ = nullptr;
+  float* d_q_ = nullptr;  // [rows, d] queries; [rows, 3d] q, K and V rows with an fp8 cache
   void* d_attn_ = nullptr;
   void* d_h_ = nullptr;
   float* d_logits_ = nullptr;

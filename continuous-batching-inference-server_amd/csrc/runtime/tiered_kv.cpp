@@ -107,8 +107,9 @@ TieredKVBlockManager::TieredKVBlockManager(int layer_count, int page_size, int n
       nvme_(nvme_scratch_path) {
   if (layer_count <= 0 || page_size <= 0 || n_heads <= 0 || head_dim <= 0)
     throw std::invalid_argument("TieredKVBlockManager: sizes must be positive");
-  if (kv_dtype != CBIS_F32 && kv_dtype != CBIS_BF16) throw std::invalid_argument("TieredKVBlockManager: kv dtype");
-  page_bytes_ = (size_t)page_size * n_heads * head_dim * dtype_size(kv_dtype);
+  if (kv_dtype != CBIS_F32 && kv_dtype != CBIS_BF16 && kv_dtype != CBIS_FP8E4M3)
+    throw std::invalid_argument("TieredKVBlockManager: kv dtype");
+  page_bytes_ = kv_page_bytes(page_size, n_heads, head_dim, kv_dtype);
   raw_block_bytes_ = (size_t)layer_count * 2 * page_bytes_;
   hip_check(hipStreamCreateWithFlags(&stream_, hipStreamNonBlocking), "TieredKVBlockManager: stream");
 }

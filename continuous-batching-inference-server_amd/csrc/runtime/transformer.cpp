@@ -80,14 +80,16 @@ TransformerRunner::TransformerRunner(const ModelWeights& weights, PagedKVCache& 
       cache.page_size() != cfg_.page_size || cache.kv_dtype() != cfg_.kv_dtype)
     throw std::invalid_argument("TransformerRunner: cache geometry does not match the model config");
   if (!cache.has_device()) throw std::invalid_argument("TransformerRunner: cache has no device pools");
-  // The attention kernels are built for head_dim 32 (any head count).
-  if (cfg_.head_dim != 32) throw std::invalid_argument("TransformerRunner: attention needs head_dim 32");
+  // The attention kernels are built for head_dim 32 (any head count), those over
+  // fp8 K/V for 32, 64 and 128 (which the config's own check covers).
+  const bool kv8 = cfg_.kv_dtype == CBIS_FP8E4M3;
+  if (cfg_.head_dim != 32 && !kv8) throw std::invalid_argument("TransformerRunner: attention needs head_dim 32");
   hip_check(hipStreamCreateWithFlags(&stream_, hipStreamNonBlocking), "hipStreamCreate");
   const size_t R = max_total_rows, D = cfg_.d_model, F = cfg_.mlp, V = cfg_.vocab;
   const size_t ae = dtype_size(cfg_.act_dtype());
   // cbis_paged_attention_proj's limits: one head block (256 fp32 / 512 bf16
   // K/V columns), a multiple of 64, at most 256 fp32 / 512 bf16 weight columns.
-  attn_proj_ok_ = D % 64 == 0 && D <= (cfg_.kv_dtype == CBIS_F32 ? 256u : 512u) &&
+  attn_proj_ok_ = !kv8 && D % 64 == 0 && D <= (cfg_.kv_dtype == CBIS_F32 ? 256u : 512u) &&
                   (cfg_.weight_dtype == CBIS_F32 ? D <= 256 : cfg_.weight_dtype == CBIS_BF16 && D <= 512);
   for (StepBuf& b : bufs_) {
     hip_check(hipEventCreate(&b.ev_start), "hipEventCreate");
@@ -101,7 +103,7 @@ TransformerRunner::TransformerRunner(const ModelWeights& weights, PagedKVCache& 
   }
   hip_check(hipMalloc((void**)&d_x_, R * D * 4), "hipMalloc x");
   hip_check(hipMalloc(&d_xn_, R * D * ae), "hipMalloc xn");
-  hip_check(hipMalloc((void**)&d_q_, R * D * 4), "hipMalloc q");
+  hip_check(hipMalloc((void**)&d_q_, R * D * 4 * (kv8 ? 3 : 1)), "hipMalloc q");
   hip_check(hipMalloc(&d_attn_, R * D * ae), "hipMalloc attn");
   hip_check(hipMalloc(&d_h_, R * F * ae), "hipMalloc h");
   hip_check(hipMalloc((void**)&d_logits_, R * V * 4), "hipMalloc logits");
@@ -111,6 +113,8 @@ TransformerRunner::TransformerRunner(const ModelWeights& weights, PagedKVCache& 
   hip_check(hipHostGetDevicePointer((void**)&hd_logits_, h_logits_, 0), "hipHostGetDevicePointer logits");
   // Split-KV partials: the automatic split keeps rows * splits <= 2048 + rows.
   ws_bytes_ = (2048 + R) * (size_t)cfg_.n_heads * (cfg_.head_dim + 4) * 4;
+  // The 8-bit calls' own splits keep rows * splits * heads <= 16384.
+  if (kv8) ws_bytes_ = (size_t)16384 * (cfg_.head_dim + 1) * 4;
   hip_check(hipMalloc(&d_ws_, ws_bytes_), "hipMalloc attention workspace");
   // Split-K workspace: the largest any of the step's GEMM shapes asks for at
   // any row count up to max_total_rows (through cbis_gemm_layernorm, whose
@@ -195,15 +199,15 @@ void TransformerRunner::prepare(int b, const int* tok, const int* pos, const int
   // Rows: runs of consecutive positions of one sequence go to the MFMA
   // prefill kernel of the K/V dtype (fp32: where that pays), everything else to
   // the split-KV decode kernel.
-  const bool bf16_kv = cfg_.kv_dtype == CBIS_BF16;
-  const int tile_rows = bf16_kv ? kTileRows : CBIS_CHUNK_TILE_ROWS, tile_ints = bf16_kv ? kTileInts : 4;
+  const bool bf16_kv = cfg_.kv_dtype == CBIS_BF16, f32_kv = cfg_.kv_dtype == CBIS_F32;
+  const int tile_rows = f32_kv ? CBIS_CHUNK_TILE_ROWS : kTileRows, tile_ints = bf16_kv ? kTileInts : 4;
   auto run_end = [&](int i) {
     int j = i + 1;
     while (j < M && seq[j] == seq[i] && pos[j] == pos[j - 1] + 1) ++j;
     return j;
   };
   bool tiles_ok = true;
-  if (!bf16_kv) {
+  if (f32_kv) {
     RowMix r;
     r.rows = M;
     for (int i = 0, j; i < M; i = j) {
@@ -292,7 +296,9 @@ void TransformerRunner::prepare(int b, const int* tok, const int* pos, const int
     const int64_t hblocks = (cfg_.n_heads + hpb - 1) / hpb;
     const int64_t rows = (int64_t)drows.size(), units = rows * hblocks;
     split_tokens_ = 0;
-    if (rows > 0 && units >= 3 * kDecodeSlots / 2 && (int64_t)max_kv * rows <= 2 * sum_kv) {
+    if (cfg_.kv_dtype == CBIS_FP8E4M3) {
+      // The 8-bit attention's own choice.
+    } else if (rows > 0 && units >= 3 * kDecodeSlots / 2 && (int64_t)max_kv * rows <= 2 * sum_kv) {
       split_tokens_ = 1 << 30;
     } else if (const int64_t share = (sum_kv * hblocks + kCUs - 1) / kCUs;
                rows > 0 && share >= 2048) {
@@ -401,6 +407,27 @@ void TransformerRunner::enqueue_forward(int b, bool greedy, bool from_prev) {
   const bool bf16_kv = cfg_.kv_dtype == CBIS_BF16;
   a.tile_pages = bf16_kv ? 8 : 0;
 
+  // fp8 K/V: the QKV GEMM leaves q, K and V rows in d_q_, the rows are quantised
+  // into their slots, and the 8-bit calls attend to them.
+  const bool kv8 = cfg_.kv_dtype == CBIS_FP8E4M3;
+  const int64_t ldqkv = 3 * (int64_t)D;
+  cbis_kv8_attn_desc a8 = {};
+  a8.n_rows = n_decode_;
+  a8.rows = d_drows_;
+  a8.n_heads = cfg_.n_heads;
+  a8.q_dtype = CBIS_F32;
+  a8.q = d_q_;
+  a8.ldq = ldqkv;
+  a8.block_table = d_bt_;
+  a8.bt_stride = bt_width_;
+  a8.row_bt = d_rowbt_;
+  a8.row_pos = d_pos_;
+  a8.out_dtype = act;
+  a8.out = d_attn_;
+  a8.ldo = D;
+  a8.workspace = d_ws_;
+  a8.workspace_bytes = ws_bytes_;
+
   // LayerNorms that follow a residual GEMM (ln2 after the out-projection,
   // the next layer's ln1 or ln_f after fc2) run with it (cbis_gemm_layernorm:
   // fused with the GEMM's split-K reduce, where it splits).  Decode-sized
@@ -423,9 +450,13 @@ void TransformerRunner::enqueue_forward(int b, bool greedy, bool from_prev) {
     g.w_dtype = wd; g.W = L.wqkv; g.ldw = D; g.w_scale = L.sqkv;
     g.bias = L.bqkv;
     g.y_dtype = CBIS_F32; g.Y = d_q_; g.ldy = D;
-    g.kv_col0 = D; g.kv_width = D; g.kv_dtype = cfg_.kv_dtype; g.page_size = cfg_.page_size;
-    g.k_pool = cache_.k_base(l); g.v_pool = cache_.v_base(l);
-    g.write_page = d_wpage_; g.write_offset = d_woff_;
+    if (kv8) {
+      g.ldy = ldqkv;
+    } else {
+      g.kv_col0 = D; g.kv_width = D; g.kv_dtype = cfg_.kv_dtype; g.page_size = cfg_.page_size;
+      g.k_pool = cache_.k_base(l); g.v_pool = cache_.v_base(l);
+      g.write_page = d_wpage_; g.write_offset = d_woff_;
+    }
     if (ln_pro) cbis_check(cbis_layernorm_gemm(&g, d_x_, D, L.ln1_w, L.ln1_b, 1e-5f, s), "ln1 + qkv gemm");
     else cbis_check(cbis_gemm(&g, s), "qkv gemm");
     a.k_pool = cache_.k_base(l);
@@ -440,7 +471,17 @@ void TransformerRunner::enqueue_forward(int b, bool greedy, bool from_prev) {
     g.w_dtype = wd; g.W = L.wo; g.ldw = D; g.w_scale = L.so;
     g.bias = L.bo; g.residual = d_x_; g.ldr = D;
     g.y_dtype = CBIS_F32; g.Y = d_x_; g.ldy = D;
-    if (fused_proj_) {
+    if (kv8) {
+      a8.cache = cache_.kv8_view(l);
+      cbis_check(cbis_kv8_scatter(&a8.cache, M, CBIS_F32, d_q_ + D, ldqkv, d_q_ + 2 * D, ldqkv, d_wpage_, d_woff_, s),
+                 "K/V rows");
+      a8.max_kv_len = max_kv_;
+      cbis_check(cbis_kv8_attention(&a8, s), "attention");
+      a8.max_kv_len = 0;  // the tiles' keys are bounded by the table's width
+      cbis_check(cbis_kv8_chunk_attention(&a8, n_tiles_, d_tiles_, s), "chunk attention");
+      if (ln_pro) cbis_check(cbis_gemm(&g, s), "out-proj gemm");
+      else cbis_check(cbis_gemm_layernorm(&g, L.ln2_w, L.ln2_b, 1e-5f, act, d_xn_, D, s), "out-proj gemm + ln2");
+    } else if (fused_proj_) {
       cbis_check(cbis_paged_attention_proj(&a, &g, s), "attention + out-proj");
     } else {
       // Single rows on the split-KV decode kernel, runs of rows on the MFMA

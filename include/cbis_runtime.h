@@ -25,7 +25,8 @@ extern "C" {
 typedef struct cbis_model_config {
   int vocab, d_model, n_heads, head_dim, n_layers, mlp, max_seq, page_size;
   int weight_dtype; /* CBIS_F32, CBIS_BF16 or CBIS_FP8E4M3 (linear weights) */
-  int kv_dtype;     /* CBIS_F32 or CBIS_BF16 (paged K/V pools) */
+  int kv_dtype;     /* CBIS_F32, CBIS_BF16 or CBIS_FP8E4M3 (paged K/V pools; fp8: the
+                       8-bit pages of cbis_kv8_cache, head_dim 32, 64 or 128) */
 } cbis_model_config;
 
 typedef struct cbis_cache cbis_cache;
@@ -157,8 +158,8 @@ typedef struct cbis_eviction_params {
 
 /* The reference's defaults (include/tiered_kv_manager.hpp:40-48). */
 void cbis_eviction_params_default(cbis_eviction_params* p);
-/* params may be NULL (defaults).  kv_dtype: CBIS_F32 (the reference's pools)
- * or CBIS_BF16. */
+/* params may be NULL (defaults).  kv_dtype: CBIS_F32 (the reference's pools),
+ * CBIS_BF16 or CBIS_FP8E4M3. */
 cbis_tiered* cbis_tiered_create(int layer_count, int page_size, int n_heads, int head_dim, int kv_dtype,
                                 const char* nvme_scratch_path, size_t gpu_capacity_blocks,
                                 size_t dram_capacity_blocks, const cbis_eviction_params* params);

@@ -126,3 +126,15 @@ def test_format_restatement():
     x[0, 3], x[1, 0] = np.nan, np.inf
     codes, byte = ref.quantise(x)
     assert (byte[:2] == 255).all() and (codes[:2] == 0).all() and np.isnan(ref.dequantise(codes, byte)[:2]).all()
+
+
+def test_host_cache_of_fp8_pages(cbis):
+    """PagedKVCache takes kv_dtype fp8 where the pages exist and refuses other
+    geometries; its bookkeeping is the other dtypes'."""
+    c = cbis.PagedKVCache(2, 8, 16, 3, 64, "fp8", alloc_device=False)
+    s = c.allocate_sequence()
+    assert c.ensure_capacity(s, 40) and c.pages(s) == [0, 1, 2] and c.num_free_pages() == 5
+    c.close()
+    for ps, hd in ((8, 32), (24, 32), (16, 48), (16, 16), (16, 256)):
+        with pytest.raises(cbis.CbisError, match="fp8 K/V pages"):
+            cbis.PagedKVCache(2, 8, ps, 3, hd, "fp8", alloc_device=False)
