@@ -467,3 +467,144 @@ def test_write_then_attend_in_a_graph(cbis, dev):
             for o in outs:
                 c.check(o[i].double().cpu().numpy().reshape(heads, d), 0, 160 + i,
                         x[i, :heads * d].astype(np.float64).reshape(heads, d), "f32", "bf16")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scatter_extremes(cbis, dev, dtype):
+    """Slices at the ends of fp32: subnormals, the largest finite values, maxima
+    just below, at and above 448 * 2^e, signed zeros; and back in both types."""
+    import torch
+    r = rng(21)
+    rows = [np.full(64, 3e-39), np.linspace(-1e-41, 1e-38, 64), r.standard_normal(64) * 3e38, np.full(64, -0.0),
+            np.full(64, np.finfo(np.float32).max), np.full(64, 1.4e-45), r.standard_normal(64) * 1e-37]
+    for e in (-126, -120, -3, 0, 5, 118):
+        for m in (1.75, np.nextafter(np.float32(1.75), np.float32(2)), np.nextafter(np.float32(1.75), np.float32(1)),
+                  1.7578125, 1.7421875, 1.0, 1.9921875):
+            x = r.standard_normal(64) * 0.3
+            x[r.integers(64)] = m
+            rows.append(np.clip(x, -m, m) * 2.0 ** (e + 8))
+    with np.errstate(over="ignore"):
+        x = np.clip(np.stack(rows), -3.38e38, 3.38e38).astype(np.float32)
+    n = len(x)
+    dx, held = _as(x, dtype, dev)
+    pools = [torch.zeros((n + 15) // 16 * ref.page_bytes(2, 32, 16), dtype=torch.uint8, device=dev) for _ in range(2)]
+    c = _cache(cbis, 2, 32, 16, *pools)
+    idx = torch.arange(n, dtype=torch.int32, device=dev)
+    page, off = idx // 16, idx % 16
+    k = cbis.kernels()
+    cbis.check(k.cbis_kv8_scatter(ctypes.byref(c), n, cbis.DTYPES[dtype], ptr(dx), 64, ptr(dx), 64, ptr(page), ptr(off),
+                                  stream()))
+    back = {d: [torch.empty((n, 64), dtype=_t(d), device=dev) for _ in range(2)] for d in ("f32", "bf16")}
+    for d, b in back.items():
+        cbis.check(k.cbis_kv8_gather(ctypes.byref(c), n, cbis.DTYPES[d], ptr(b[0]), 64, ptr(b[1]), 64, ptr(page),
+                                     ptr(off), stream()))
+    sync()
+    codes, byte = ref.quantise(held.reshape(n, 2, 32))
+    exact = ref.dequantise(codes, byte).reshape(n, 64)
+    for w in range(2):
+        got = pools[w].cpu().numpy()
+        want = np.zeros_like(got)
+        for i in range(n):
+            ref.store(want, w == 1, 2, 32, 16, i // 16, i % 16, held[i].reshape(2, 32))
+        assert np.array_equal(got, want), "KV"[w]
+        for d, b in back.items():
+            with np.errstate(over="ignore"):
+                stored = torch.from_numpy(exact.astype(np.float32)).to(_t(d)).double().numpy()
+            assert np.array_equal(b[w].double().cpu().numpy(), stored), ("KV"[w], d)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(16, 2, 32), (12, 1, 32), (24, 2, 64), (64, 2, 128), (9, 9, 32)])
+@pytest.mark.parametrize("q_dtype,out_dtype", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+def test_attention_other_groups(cbis, dev, heads, kv_heads, d, q_dtype, out_dtype):
+    """Groups of 8, 12, 16 and 32 query heads (one, two or four kv heads to a
+    workgroup's columns), every number of waves on a row, 128-token pages, V
+    slices over 20 binades; both forms agree with 64 bits."""
+    import torch
+    c = Case(cbis, dev, kv_heads, d, 128, [700, 31], seed=heads, spread=10)
+    w = heads * d
+    n = 9
+    q, qv = _as(rng(8).standard_normal((n, w)).astype(np.float32), q_dtype, dev)
+    seq = np.array([0, 0, 1, 0, 1, 0, 0, 0, 0], np.int32)
+    pos = np.array([699, 63, 30, 64, 0, 128, 250, 575, -1], np.int32)
+    d_seq, d_pos = torch.from_numpy(seq).to(dev), torch.from_numpy(pos).to(dev)
+    k = cbis.kernels()
+    for split in (0, 64, 128, 192, 256, 512):
+        out = torch.full((n, w), 7.0, dtype=_t(out_dtype), device=dev)
+        a = c.desc(cbis, q, q_dtype, out, out_dtype, heads)
+        a.n_rows, a.row_bt, a.row_pos, a.max_kv_len, a.split_tokens = n, ptr(d_seq), ptr(d_pos), 700, split
+        ws = _workspace(a, k.cbis_kv8_attention_workspace_size(ctypes.byref(a)), dev)
+        cbis.check(k.cbis_kv8_attention(ctypes.byref(a), stream()))
+        sync()
+        got = out.double().cpu().numpy().reshape(n, heads, d)
+        for i in range(n):
+            c.check(got[i], seq[i], pos[i], qv[i].reshape(heads, d), q_dtype, out_dtype, f"decode split {split}")
+        tiles = torch.tensor([(0, 9, 0, 691)], dtype=torch.int32, device=dev)
+        a.n_rows = 0
+        ws = _workspace(a, k.cbis_kv8_chunk_attention_workspace_size(ctypes.byref(a), 1), dev)
+        cbis.check(k.cbis_kv8_chunk_attention(ctypes.byref(a), 1, ptr(tiles), stream()))
+        sync()
+        del ws
+        got = out.double().cpu().numpy().reshape(n, heads, d)
+        for i in (0, 4, 8):
+            c.check(got[i], 0, 691 + i, qv[i].reshape(heads, d), q_dtype, out_dtype, f"chunk split {split}")
+
+
+def test_many_rows_and_tiles(cbis, dev):
+    """Enough rows and tiles that waves no longer share keys: 700 rows of 8 heads
+    of 32 (one wave to a row's heads), and the same rows as tiles."""
+    import torch
+    c = Case(cbis, dev, 8, 32, 16, [700], seed=33)
+    q, qv = _as(rng(3).standard_normal((700, 256)).astype(np.float32), "f32", dev)
+    pos = torch.arange(700, dtype=torch.int32, device=dev)
+    many = pos.repeat(8)
+    zero = torch.zeros(5600, dtype=torch.int32, device=dev)
+    rows = (torch.arange(5600, dtype=torch.int32, device=dev) % 700).contiguous()
+    tiles = torch.tensor([(at, min(64, 700 - at), 0, at) for at in range(0, 700, 64)] * 12, dtype=torch.int32, device=dev)
+    k = cbis.kernels()
+    for form in ("decode", "chunk"):
+        out = torch.empty((700, 256), dtype=torch.bfloat16, device=dev)
+        a = c.desc(cbis, q, "f32", out, "bf16", 8)
+        a.row_bt, a.row_pos, a.max_kv_len = ptr(zero), ptr(many), 700
+        if form == "decode":
+            a.n_rows, a.rows = 5600, ptr(rows)
+            assert k.cbis_kv8_attention_workspace_size(ctypes.byref(a)) == 0
+            cbis.check(k.cbis_kv8_attention(ctypes.byref(a), stream()))
+        else:
+            assert k.cbis_kv8_chunk_attention_workspace_size(ctypes.byref(a), len(tiles)) == 0
+            cbis.check(k.cbis_kv8_chunk_attention(ctypes.byref(a), len(tiles), ptr(tiles), stream()))
+        sync()
+        got = out.double().cpu().numpy().reshape(700, 8, 32)
+        for i in (0, 15, 16, 63, 64, 300, 639, 640, 699):
+            c.check(got[i], 0, i, qv[i].reshape(8, 32), "f32", "bf16", form)
+
+
+def test_two_streams(cbis, dev):
+    """Two attention calls with splits at once on two streams, each with its own
+    workspace: the results of the calls alone, bit for bit."""
+    import torch
+    c = Case(cbis, dev, 4, 64, 16, [500, 300], seed=17)
+    k = cbis.kernels()
+    calls = []
+    for i in range(2):
+        q, _ = _as(rng(40 + i).standard_normal((30, 8 * 64)).astype(np.float32), "f32", dev)
+        out = torch.empty((30, 8 * 64), device=dev)
+        seq = torch.full((30,), i, dtype=torch.int32, device=dev)
+        pos = torch.arange(200, 230, dtype=torch.int32, device=dev)
+        a = c.desc(cbis, q, "f32", out, "f32", 8)
+        a.n_rows, a.row_bt, a.row_pos, a.split_tokens, a.max_kv_len = 30, ptr(seq), ptr(pos), 64, 230
+        ws = _workspace(a, k.cbis_kv8_attention_workspace_size(ctypes.byref(a)), dev)
+        calls.append((a, out, (q, seq, pos, ws)))
+    alone = []
+    for a, out, _ in calls:
+        cbis.check(k.cbis_kv8_attention(ctypes.byref(a), stream()))
+        sync()
+        alone.append(out.clone())
+        out.zero_()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sync()
+    for _ in range(5):
+        for (a, _, _), s in zip(calls, streams):
+            cbis.check(k.cbis_kv8_attention(ctypes.byref(a), s.cuda_stream))
+    sync()
+    for (_, out, _), want in zip(calls, alone):
+        assert torch.equal(out, want)
