@@ -415,9 +415,9 @@ struct AttnArgs {
   int n_tiles, ncg;  // column groups of a kv head
 };
 
-// 8 consecutive q values of a column as QP bf16 parts.
+// 8 consecutive q values of a column, times scale, as QP bf16 parts.
 template <int QP>
-__device__ inline void load_q8(const AttnArgs& a, int64_t at, bool valid, bf16v8_t* part) {
+__device__ inline void load_q8(const AttnArgs& a, int64_t at, bool valid, float scale, bf16v8_t* part) {
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = 0.f;
@@ -445,6 +445,8 @@ __device__ inline void load_q8(const AttnArgs& a, int64_t at, bool valid, bf16v8
       }
     }
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= scale;
 #pragma unroll
   for (int k = 0; k < QP; ++k)
 #pragma unroll
@@ -611,7 +613,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
   bf16v8_t q[NK][QP];
 #pragma unroll
   for (int s = 0; s < NK; ++s)
-    load_q8<QP>(a, (int64_t)row * a.ldq + (int64_t)(h0 + n) * HD + q_dim<HD>(s, g), col_ok, q[s]);
+    load_q8<QP>(a, (int64_t)row * a.ldq + (int64_t)(h0 + n) * HD + q_dim<HD>(s, g), col_ok, 1.f, q[s]);
 
   float m = kLowest, l = 0.f;
   int E = 0;
@@ -855,6 +857,59 @@ constexpr int kChunkCols = 32;  // columns of a wave at head_dim 32
 // and take 200 us, 16 101).
 constexpr int chunk_cols(int hd, int qp) { return hd == 128 && qp == 3 ? 16 : kChunkCols; }
 
+// Scores that come out of the products as log2 units against the running
+// reference, s - m + 8, the sums' initial value being 8 - m and q scaled on the way
+// in: no instruction per score to scale it and to subtract m.  Not for bf16 q,
+// which one part holds exactly as it is, but not scaled.
+constexpr bool relative_scores(int qp) { return qp > 1; }
+
+template <bool kRel>
+__device__ inline f32x4_t first_sums(float m) {
+  const float x = kRel ? 8.f - m : 0.f;
+  return f32x4_t{x, x, x, x};
+}
+
+// Raises a column's reference m to the block's maximum where that passes it by
+// more than 2^7, and what was summed against the old one with it.
+template <bool kRel, int ND, int CT>
+__device__ inline void raise_reference(f32x4_t (&S)[4][CT], f32x4_t (&O)[ND][CT], f32x4_t (&l)[CT], float (&m)[CT],
+                                       float qscale, bool fresh) {
+  float top[CT];
+  bool grow = kRel && fresh;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    top[ct] = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[ct] = fmaxf(top[ct], S[p][ct][i]);
+    if constexpr (!kRel) top[ct] *= qscale;
+    grow |= kRel ? top[ct] > 15.f : top[ct] > m[ct] + 7.f;
+  }
+  if (!__ballot(grow)) return;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const float t = column_max(top[ct]);
+    float r, m1;
+    if constexpr (kRel) {
+      // In the first block the reference may also fall (a column that sees
+      // nothing of it sees nothing of the later ones either).
+      const float up = fresh ? (t == -INFINITY ? 0.f : t - 8.f) : fmaxf(t - 8.f, 0.f);
+      r = fresh ? 1.f : fast_exp2(-up);
+      m1 = m[ct] + up;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) S[p][ct] -= up;
+    } else {
+      m1 = fmaxf(m[ct], t);
+      r = fast_exp2(m[ct] - m1);
+    }
+    l[ct] *= r;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) O[i][ct] *= r;
+    m[ct] = m1;
+  }
+}
+
 template <int HD>
 struct ChunkStage {
   static constexpr int KG = 128 / HD;
@@ -876,6 +931,7 @@ constexpr size_t chunk_lds(int waves) {
 template <int HD, int SW, int QP, int PP>
 __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
   constexpr int NK = HD / 32, ND = HD / 16, KG = 128 / HD, W = 8 / SW, WH = W / KG, COLS = chunk_cols(HD, QP), CT = COLS / 16;
+  constexpr bool kRel = relative_scores(QP);
   extern __shared__ __align__(16) char lds[];
   ChunkStage<HD>* stage = (ChunkStage<HD>*)lds;
   _Float16(*factor)[64] = (_Float16(*)[64])(lds + 2 * sizeof(ChunkStage<HD>));  // a wave's own, of the block it stages
@@ -907,18 +963,19 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
     pos[ct] = ok ? min(pos0 + t, a.max_tok - 1) : -1;
 #pragma unroll
     for (int s = 0; s < NK; ++s)
-      load_q8<QP>(a, (int64_t)(row0 + t) * a.ldq + (int64_t)head * HD + q_dim<HD>(s, g), ok, q[ct][s]);
+      load_q8<QP>(a, (int64_t)(row0 + t) * a.ldq + (int64_t)head * HD + q_dim<HD>(s, g), ok, kRel ? a.qscale : 1.f, q[ct][s]);
   }
   float m[CT];
   int E = 0;
   f32x4_t O[ND][CT], l[CT];  // l: every lane of a column holds its sum four times over
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    m[ct] = kLowest;
+    m[ct] = kRel ? 0.f : kLowest;
     l[ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < ND; ++i) O[i][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
+  bool fresh = true;  // no block yet: the reference is the first one's maximum
   f16v8_t ones;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (_Float16)1.f;
@@ -1017,7 +1074,7 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
 #pragma unroll
       for (int p = 0; p < 4; ++p)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) S[p][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int ct = 0; ct < CT; ++ct) S[p][ct] = first_sums<kRel>(m[ct]);
       // Operand y is product op_p(y), k step op_s(y): products alternate, so that no
       // two instructions in a row wait for the same sums.
       auto op_p = [](int y) { return y / (2 * NK) * 2 + (y & 1); };
@@ -1082,29 +1139,8 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
           for (int i = 0; i < ND; ++i) O[i][ct] *= r;
         E = E1;
       }
-      float top[CT];
-      bool grow = false;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        top[ct] = -INFINITY;
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top[ct] = fmaxf(top[ct], S[p][ct][i]);
-        top[ct] *= a.qscale;
-        grow |= top[ct] > m[ct] + 7.f;
-      }
-      if (__ballot(grow)) {
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          const float m1 = fmaxf(m[ct], column_max(top[ct]));
-          const float r = fast_exp2(m[ct] - m1);
-          l[ct] *= r;
-#pragma unroll
-          for (int i = 0; i < ND; ++i) O[i][ct] *= r;
-          m[ct] = m1;
-        }
-      }
+      raise_reference<kRel, ND, CT>(S, O, l, m, a.qscale, fresh);
+      fresh = false;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         f16v8_t P[CT][PP];
@@ -1114,7 +1150,7 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
           for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              float x = fast_exp2(S[2 * half + h][ct][i] * a.qscale - (m[ct] - 8.f));
+              float x = fast_exp2(kRel ? S[2 * half + h][ct][i] : S[2 * half + h][ct][i] * a.qscale - (m[ct] - 8.f));
 #pragma unroll
               for (int k = 0; k < PP; ++k) {
                 const _Float16 y = (_Float16)x;
@@ -1210,6 +1246,7 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
 template <int QP, int PP>
 __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const AttnArgs a) {
   constexpr int HD = 32, ND = 2, CT = kChunkCols / 16, kPitch = HD + 4;
+  constexpr bool kRel = relative_scores(QP);
   // Per wave 64 V factors of the block at hand; at the end the parts' results.
   extern __shared__ __align__(16) char lds[];
   const int wave = wave_id(), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
@@ -1236,18 +1273,19 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const At
     const int c = c0 + 16 * ct + n, t = c / a.group, head = kh * a.group + c % a.group;
     const bool ok = busy && c < cols;
     pos[ct] = ok ? min(pos0 + t, a.max_tok - 1) : -1;
-    load_q8<QP>(a, (int64_t)(row0 + t) * a.ldq + (int64_t)head * HD + q_dim<HD>(0, g), ok, q[ct]);
+    load_q8<QP>(a, (int64_t)(row0 + t) * a.ldq + (int64_t)head * HD + q_dim<HD>(0, g), ok, kRel ? a.qscale : 1.f, q[ct]);
   }
   float m[CT];
   int E = 0;
   f32x4_t O[ND][CT], l[CT];  // l: every lane of a column holds its sum four times over
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    m[ct] = kLowest;
+    m[ct] = kRel ? 0.f : kLowest;
     l[ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < ND; ++i) O[i][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
+  bool fresh = true;  // no block yet: the reference is the first one's maximum
   f16v8_t ones;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (_Float16)1.f;
@@ -1290,7 +1328,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const At
         const bf16v8_t kf = codes_bf16(kr[p].w[0], kr[p].w[1], ks);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          S[p][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          S[p][ct] = first_sums<kRel>(m[ct]);
 #pragma unroll
           for (int k = 0; k < QP; ++k)
             S[p][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[ct][k], S[p][ct], 0, 0, 0);
@@ -1337,29 +1375,8 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const At
         E = E1;
       }
       factor[lane] = (_Float16)ldexpf(1.f, byte - E + 6);
-      float top[CT];
-      bool grow = false;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        top[ct] = -INFINITY;
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top[ct] = fmaxf(top[ct], S[p][ct][i]);
-        top[ct] *= a.qscale;
-        grow |= top[ct] > m[ct] + 7.f;
-      }
-      if (__ballot(grow)) {
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          const float m1 = fmaxf(m[ct], column_max(top[ct]));
-          const float r = fast_exp2(m[ct] - m1);
-          l[ct] *= r;
-#pragma unroll
-          for (int i = 0; i < ND; ++i) O[i][ct] *= r;
-          m[ct] = m1;
-        }
-      }
+      raise_reference<kRel, ND, CT>(S, O, l, m, a.qscale, fresh);
+      fresh = false;
       if ((b + 1) * kBlk > kv) {  // a slot past the last key may hold anything
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
@@ -1377,7 +1394,8 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const At
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            float x = fast_exp2(S[2 * half + i / 4][ct][i & 3] * a.qscale - (m[ct] - 8.f));
+            const float y0 = S[2 * half + i / 4][ct][i & 3];
+            float x = fast_exp2(kRel ? y0 : y0 * a.qscale - (m[ct] - 8.f));
 #pragma unroll
             for (int k = 0; k < PP; ++k) {
               const _Float16 y = (_Float16)x;
