@@ -870,12 +870,14 @@ __device__ inline f32x4_t first_sums(float m) {
 }
 
 // Raises a column's reference m to the block's maximum where that passes it by
-// more than 2^7, and what was summed against the old one with it.
+// more than 2^7, and what was summed against the old one with it.  fresh: the
+// column has met no score yet (above -inf); it stays so only where more keys follow,
+// its last one being pos and the next block's first one `next`.
 template <bool kRel, int ND, int CT>
 __device__ inline void raise_reference(f32x4_t (&S)[4][CT], f32x4_t (&O)[ND][CT], f32x4_t (&l)[CT], float (&m)[CT],
-                                       float qscale, bool fresh) {
+                                       float qscale, bool (&fresh)[CT], const int (&pos)[CT], int next) {
   float top[CT];
-  bool grow = kRel && fresh;
+  bool grow = false;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     top[ct] = -INFINITY;
@@ -884,7 +886,7 @@ __device__ inline void raise_reference(f32x4_t (&S)[4][CT], f32x4_t (&O)[ND][CT]
 #pragma unroll
       for (int i = 0; i < 4; ++i) top[ct] = fmaxf(top[ct], S[p][ct][i]);
     if constexpr (!kRel) top[ct] *= qscale;
-    grow |= kRel ? top[ct] > 15.f : top[ct] > m[ct] + 7.f;
+    grow |= kRel ? fresh[ct] || top[ct] > 15.f : top[ct] > m[ct] + 7.f;
   }
   if (!__ballot(grow)) return;
 #pragma unroll
@@ -892,11 +894,11 @@ __device__ inline void raise_reference(f32x4_t (&S)[4][CT], f32x4_t (&O)[ND][CT]
     const float t = column_max(top[ct]);
     float r, m1;
     if constexpr (kRel) {
-      // In the first block the reference may also fall (a column that sees
-      // nothing of it sees nothing of the later ones either).
-      const float up = fresh ? (t == -INFINITY ? 0.f : t - 8.f) : fmaxf(t - 8.f, 0.f);
-      r = fresh ? 1.f : fast_exp2(-up);
+      // The first reference may also be a lower one than the initial 0.
+      const float up = fresh[ct] ? (t == -INFINITY ? 0.f : t - 8.f) : fmaxf(t - 8.f, 0.f);
+      r = fresh[ct] ? 1.f : fast_exp2(-up);
       m1 = m[ct] + up;
+      fresh[ct] = fresh[ct] && t == -INFINITY && pos[ct] >= next;
 #pragma unroll
       for (int p = 0; p < 4; ++p) S[p][ct] -= up;
     } else {
@@ -943,9 +945,10 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
   unit /= (unsigned)a.c.kv_heads;
   const int split = (int)(unit % (unsigned)a.nsplit);
   const int64_t tile = unit / (unsigned)a.nsplit;
-  // Tiles are handed over as cbis_paged_prefill_attention's: row, rows, table row, position.
+  // Tiles are handed over as cbis_paged_prefill_attention's: row, rows, table row,
+  // position (past the table all are alike: every key it covers).
   const int row0 = a.tiles[4 * tile], nv = min(a.tiles[4 * tile + 1], CBIS_PREFILL_TILE_ROWS),
-            btr = a.tiles[4 * tile + 2], pos0 = a.tiles[4 * tile + 3];
+            btr = a.tiles[4 * tile + 2], pos0 = min(a.tiles[4 * tile + 3], a.max_tok);
   const int cols = nv * a.group, wg0 = cg * WH * COLS;
   if (wg0 >= cols) return;
   const int* bt = a.bt + (int64_t)btr * a.bt_stride;
@@ -966,16 +969,17 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
       load_q8<QP>(a, (int64_t)(row0 + t) * a.ldq + (int64_t)head * HD + q_dim<HD>(s, g), ok, kRel ? a.qscale : 1.f, q[ct][s]);
   }
   float m[CT];
+  bool fresh[CT];
   int E = 0;
   f32x4_t O[ND][CT], l[CT];  // l: every lane of a column holds its sum four times over
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     m[ct] = kRel ? 0.f : kLowest;
+    fresh[ct] = true;
     l[ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < ND; ++i) O[i][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  bool fresh = true;  // no block yet: the reference is the first one's maximum
   f16v8_t ones;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (_Float16)1.f;
@@ -1139,8 +1143,7 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
           for (int i = 0; i < ND; ++i) O[i][ct] *= r;
         E = E1;
       }
-      raise_reference<kRel, ND, CT>(S, O, l, m, a.qscale, fresh);
-      fresh = false;
+      raise_reference<kRel, ND, CT>(S, O, l, m, a.qscale, fresh, pos, (b + 1) * kBlk);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         f16v8_t P[CT][PP];
@@ -1260,7 +1263,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const At
   const int tile = (int)(unit / (unsigned)a.nsplit);
   const bool in = tile < a.n_tiles;
   const int4 td = in ? *(const int4*)(a.tiles + 4 * (int64_t)tile) : make_int4(0, 0, 0, 0);
-  const int row0 = td.x, nv = min(td.y, CBIS_PREFILL_TILE_ROWS), pos0 = td.w;
+  const int row0 = td.x, nv = min(td.y, CBIS_PREFILL_TILE_ROWS), pos0 = min(td.w, a.max_tok);
   const int c0 = cg * kChunkCols, cols = nv * a.group;
   const bool busy = in && c0 < cols;
   const int* bt = a.bt + (int64_t)td.z * a.bt_stride;
@@ -1276,16 +1279,17 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const At
     load_q8<QP>(a, (int64_t)(row0 + t) * a.ldq + (int64_t)head * HD + q_dim<HD>(0, g), ok, kRel ? a.qscale : 1.f, q[ct]);
   }
   float m[CT];
+  bool fresh[CT];
   int E = 0;
   f32x4_t O[ND][CT], l[CT];  // l: every lane of a column holds its sum four times over
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     m[ct] = kRel ? 0.f : kLowest;
+    fresh[ct] = true;
     l[ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < ND; ++i) O[i][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  bool fresh = true;  // no block yet: the reference is the first one's maximum
   f16v8_t ones;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (_Float16)1.f;
@@ -1375,8 +1379,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const At
         E = E1;
       }
       factor[lane] = (_Float16)ldexpf(1.f, byte - E + 6);
-      raise_reference<kRel, ND, CT>(S, O, l, m, a.qscale, fresh);
-      fresh = false;
+      raise_reference<kRel, ND, CT>(S, O, l, m, a.qscale, fresh, pos, (b + 1) * kBlk);
       if ((b + 1) * kBlk > kv) {  // a slot past the last key may hold anything
 #pragma unroll
         for (int d = 0; d < 4; ++d) {

@@ -608,3 +608,72 @@ def test_two_streams(cbis, dev):
     sync()
     for (_, out, _), want in zip(calls, alone):
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 8, 32), (8, 4, 64), (8, 2, 128)])
+def test_positions_past_the_table(cbis, dev, heads, kv_heads, d):
+    """A position past the table's 48 tokens, up to the largest int, reads those 48."""
+    import torch
+    c = Case(cbis, dev, kv_heads, d, 16, [48], seed=51)
+    w, top = heads * d, 2**31 - 1
+    q, qv = _as(rng(52).standard_normal((6, w)).astype(np.float32), "f32", dev)
+    pos = torch.tensor([47, 48, 49, 4000, top - 1, top], dtype=torch.int32, device=dev)
+    zero = torch.zeros(6, dtype=torch.int32, device=dev)
+    tiles = torch.tensor([(0, 1, 0, 47), (1, 2, 0, 48), (3, 1, 0, 4000), (4, 2, 0, top)], dtype=torch.int32, device=dev)
+    k = cbis.kernels()
+    for form in ("decode", "chunk"):
+        out = torch.empty((6, w), device=dev)
+        a = c.desc(cbis, q, "f32", out, "f32", heads)
+        a.bt_stride, a.n_rows, a.row_bt, a.row_pos = 3, 6, ptr(zero), ptr(pos)
+        if form == "decode":
+            ws = _workspace(a, k.cbis_kv8_attention_workspace_size(ctypes.byref(a)), dev)
+            cbis.check(k.cbis_kv8_attention(ctypes.byref(a), stream()))
+        else:
+            ws = _workspace(a, k.cbis_kv8_chunk_attention_workspace_size(ctypes.byref(a), 4), dev)
+            cbis.check(k.cbis_kv8_chunk_attention(ctypes.byref(a), 4, ptr(tiles), stream()))
+        sync()
+        del ws
+        got = out.double().cpu().numpy().reshape(6, heads, d)
+        for i in range(6):
+            c.check(got[i], 0, 47, qv[i].reshape(heads, d), "f32", "f32", form)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 8, 32), (8, 4, 64), (8, 2, 128)])
+@pytest.mark.parametrize("q_dtype,out_dtype", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+def test_first_scores_of_minus_infinity(cbis, dev, heads, kv_heads, d, q_dtype, out_dtype):
+    """The first 64 keys' scores fall below fp32's range (weight 0), the others' lie
+    far below 0 themselves: their softmax is what comes out."""
+    import torch
+    c = Case(cbis, dev, kv_heads, d, 16, [164], seed=61)
+    pool = c.pools[0].cpu().numpy()
+    for t in range(164):
+        x = np.full((kv_heads, d), -2.0**100 if t < 64 else -2.0**-25, np.float32)
+        if t >= 64:  # the scores of the others differ by up to 32 * 3 / 8 / sqrt(d)
+            x[:, 0] *= 1 + t % 4 / 8
+        ref.store(pool, False, kv_heads, d, 16, c.table[0, t // 16], t % 16, x)
+        c.kv[0][0][t] = ref.fetch(pool, False, kv_heads, d, 16, c.table[0, t // 16], t % 16)
+    c.pools[0].copy_(torch.from_numpy(pool))
+    w = heads * d
+    q, qv = _as(np.full((64, w), 2.0**30, np.float32), q_dtype, dev)
+    pos = torch.arange(100, 164, dtype=torch.int32, device=dev)
+    zero = torch.zeros(64, dtype=torch.int32, device=dev)
+    tiles = torch.tensor([(0, 64, 0, 100)], dtype=torch.int32, device=dev)
+    k = cbis.kernels()
+    for form, split in (("decode", 0), ("decode", 64), ("chunk", 0), ("chunk", 64)):
+        out = torch.empty((64, w), dtype=_t(out_dtype), device=dev)
+        a = c.desc(cbis, q, q_dtype, out, out_dtype, heads)
+        a.n_rows, a.row_bt, a.row_pos, a.split_tokens, a.max_kv_len = 64, ptr(zero), ptr(pos), split, 164
+        if form == "decode":
+            ws = _workspace(a, k.cbis_kv8_attention_workspace_size(ctypes.byref(a)), dev)
+            cbis.check(k.cbis_kv8_attention(ctypes.byref(a), stream()))
+        else:
+            ws = _workspace(a, k.cbis_kv8_chunk_attention_workspace_size(ctypes.byref(a), 1), dev)
+            cbis.check(k.cbis_kv8_chunk_attention(ctypes.byref(a), 1, ptr(tiles), stream()))
+        sync()
+        del ws
+        got = out.double().cpu().numpy().reshape(64, heads, d)
+        for i in (0, 27, 28, 40, 63):
+            kk, vv = (x[64:100 + i + 1] for x in c.kv[0])
+            want, mag, big = ref.attend(qv[i].reshape(heads, d), kk, vv)
+            tol = ref.tolerance(want, mag, big, 101 + i, d, np.abs(c.kv[0][1]).max(), q_dtype, out_dtype)
+            assert (np.abs(got[i] - want) <= tol).all(), (form, split, i)
