@@ -1481,6 +1481,8 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const At
 // their sums.  HD / 4 lanes hold 4 dims each; `share` such groups of a wave (a
 // power of two) take a (slot, head)'s splits in turn, a slot being a decode row
 // or a tile's row.
+constexpr int kMergeAhead = 4;  // splits whose loads a lane has on their way
+
 template <int HD>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(const AttnArgs a, int64_t slots, int share) {
   constexpr int L = HD / 4;
@@ -1502,16 +1504,25 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const AttnArgs a, int64_
   // Each group's own running maximum, its sum and its weighted outputs.
   float top = -INFINITY, sum = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = lane % w / L; ok && s < a.nsplit; s += share) {
-    const int64_t at = first + (int64_t)s * a.n_heads;
-    const float ls = a.lse[at];
-    const f32x4_t x = *(const f32x4_t*)(a.part + at * HD + d);
-    if (ls == -INFINITY) continue;  // an empty split; its outputs may not be there
-    const float t1 = fmaxf(top, ls);
-    const float f0 = fast_exp2(top - t1), f1 = fast_exp2(ls - t1);
-    sum = sum * f0 + f1;
-    o = o * f0 + x * f1;
-    top = t1;
+  for (int s0 = lane % w / L; ok && s0 < a.nsplit; s0 += kMergeAhead * share) {
+    float ls[kMergeAhead];
+    f32x4_t x[kMergeAhead];
+#pragma unroll
+    for (int u = 0; u < kMergeAhead; ++u) {
+      const int s = s0 + u * share;
+      const int64_t at = first + (int64_t)min(s, a.nsplit - 1) * a.n_heads;
+      ls[u] = s < a.nsplit ? a.lse[at] : -INFINITY;
+      x[u] = *(const f32x4_t*)(a.part + at * HD + d);
+    }
+#pragma unroll
+    for (int u = 0; u < kMergeAhead; ++u) {
+      if (ls[u] == -INFINITY) continue;  // an empty split; its outputs may not be there
+      const float t1 = fmaxf(top, ls[u]);
+      const float f0 = fast_exp2(top - t1), f1 = fast_exp2(ls[u] - t1);
+      sum = sum * f0 + f1;
+      o = o * f0 + x[u] * f1;
+      top = t1;
+    }
   }
   float all = top;
   for (int x = L; x < w; x *= 2) all = fmaxf(all, __shfl_xor(all, x, 64));
@@ -1601,6 +1612,8 @@ int kv8_rows(bool gather, const cbis_kv8_cache* c, int n_rows, int dtype, const 
   return check_launch(who);
 }
 
+constexpr int64_t kCUs = 256;
+
 // Sizes that both the workspace queries and the launches go by.
 struct Plan {
   int nsplit = 1, split_blocks = 1 << 24;
@@ -1655,16 +1668,26 @@ Plan plan_decode(const cbis_kv8_attn_desc* d) {
   //   64 rows of 1000 x 64 heads of 32 (1024)                    1: 48   2: 47   4: 50   8: 62
   //   61 rows of 500..16384, 32 / 8 heads of 128 (488)           1: 563  2: 319  4: 230  8: 193
   //   16 rows of 1000 x 64 heads of 32 (256)                     1: 37   2: 23   4: 16   8: 17
-  // Past eight waves the keys are split over workgroups, of at least 16 blocks
-  // (a join costs a launch; 1 row of 16384, 8 kv heads of 128: 4 blocks 35 us, 8
-  // 25, 16 25, 32 29; 16 rows of 32768 x 64 heads: 64 blocks 358, 128 357, 256 345).
+  // Past eight waves the keys are split over workgroups of eight, a CU's worth.
+  // Up to 64 head blocks make one round of 256 workgroups, whose rows' lengths
+  // matter little; more of them two rounds, since the rest of a GPU that is half
+  // full is lost where the rows are uneven.  us by tokens of a split, equal rows /
+  // rows of any length up to that (* what the rule takes):
+  //   4 rows of 16384, 8 kv heads of 128   1024: 45 / 39  2048*: 35 / 31  4096: 50 / 43
+  //   8 rows of 16384                      2048: 66 / 53  4096*: 57 / 50  8192: 86 / 73
+  //   16 rows of 16384                     4096*: 109 / 79  8192: 100 / 84
+  //   24 rows of 16384                     8192*: - / 93  16384: - / 134
+  //   1 row of 4000, 64 heads of 32        256*: 12.4  512: 14.9  1024: 17  4096: 28
+  // A row of 600 is faster whole (10.2; 256: 10.9), one of 1000 in splits (12.2; 11.0).
   const int64_t units = std::max<int64_t>(1, p.slots * p.nhb), blocks = longest(d);
   const int64_t part = d->split_tokens > 0 ? std::min<int64_t>(blocks, d->split_tokens / kBlk) : blocks;
   while (p.tw < kDecodeWaves && units * p.tw < 4096 && p.tw < part) p.tw *= 2;
   p.waves = std::max(p.tw, 4);
   p.groups = (int)cdiv(p.nhb, p.waves / p.tw);
-  const int64_t n = std::max<int64_t>(1, 4096 / (units * kDecodeWaves));
-  set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, n), 16), &p);
+  int64_t per = blocks;
+  if (units <= 64 && blocks >= 16) per = std::max<int64_t>(cdiv(blocks, kCUs / units), 4);
+  else if (units <= kCUs && blocks >= 16) per = std::max<int64_t>(cdiv(blocks, 2 * kCUs / units), 16);
+  set_splits(d, blocks, per, &p);
   return p;
 }
 
@@ -1685,7 +1708,12 @@ Plan plan_chunk(const cbis_kv8_attn_desc* d, int n_tiles) {
     //   16 rows after 32000                      1: 118   2048: 61    4096: 61    8192: 61
     while (p.tw < kDecodeWaves && units * p.tw < 2048 && p.tw < part) p.tw *= 2;
     p.waves = std::max(p.tw, 4);
-    set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, 4096 / (units * kDecodeWaves))), 16), &p);
+    // Splits for one workgroup of eight per CU, from 48 blocks on.  us by tokens of
+    // a split (* the rule's): 64 rows of 64 heads after 2000  1024: 19  2048*: 14,
+    // after 4000  1024: 22  2048*: 18  4096: 20, after 32000  8192: 64  16384*: 60
+    // 32768: 93; 64 rows of 8 heads after 4000  256*: 11.4  1024: 14  4096: 19.
+    if (blocks >= 48) set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, kCUs / units)), 4), &p);
+    else set_splits(d, blocks, blocks, &p);
     return p;
   }
   // As many waves as a kv head's columns fill, times the parts of the keys, up to 8.
@@ -1696,9 +1724,19 @@ Plan plan_chunk(const cbis_kv8_attn_desc* d, int n_tiles) {
   const int wh = 8 / p.sw / KG;
   p.ncg = (want + wh - 1) / wh;
   const int64_t units = std::max<int64_t>(1, (int64_t)n_tiles * d->cache.n_kv_heads * p.ncg);
-  // Splits for one workgroup per CU (512 rows after 16384, 32 / 8 heads of 128: 4
-  // splits 174 us, 8 175 and another 9 us of joining).
-  set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, 256 / units)), 8 * KG), &p);
+  // Splits for one workgroup per CU, of at least sqrt(blocks) / 2 blocks: more of
+  // them cost more to join than they save.  us by tokens of a split (* the rule's):
+  //   32 / 8 heads of 128, 512 rows after 16384  4 splits* 174, 8 175 and another 9 us of joining
+  //     64 rows after 300    64: 15.6  128*: 17  512: 21     after 1000  64: 21  128*: 20  256: 22  512: 29
+  //     64 rows after 4096   128: 37  256*: 28  512: 33      256 rows after 500  64: 36  128*: 25  512: 33
+  //   16 / 4 heads of 64, 64 rows after 4096  128: 22  256*: 17  512: 19   after 300  128: 12.4  whole*: 11.9
+  int64_t per = blocks;
+  if (blocks > 4 * KG) {
+    per = KG;
+    while (4 * per * per < blocks) per += KG;
+    per = std::max<int64_t>({per, 2, cdiv(blocks, std::max<int64_t>(1, kCUs / units))});
+  }
+  set_splits(d, blocks, per, &p);
   return p;
 }
 
