@@ -1716,10 +1716,21 @@ Plan plan_chunk(const cbis_kv8_attn_desc* d, int n_tiles) {
     else set_splits(d, blocks, blocks, &p);
     return p;
   }
-  // As many waves as a kv head's columns fill, times the parts of the keys, up to 8.
+  // As many waves as a kv head's columns fill, times the parts of the keys: up to 8,
+  // or 4 where the longest row has no more than 32 blocks: smaller pieces, two to a
+  // CU, even out the tiles' lengths, but each converts K and V for itself.  us with
+  // 8 / 4 waves:
+  //   32 / 8 heads of 128  512 fresh rows 27 / 23  64 after 1000 20 / 19  1500 after 300 69 / 63
+  //     512 after 4096 67 / 80  4 x 512 after 8192 298 / 324  8192 fresh rows 571 / 584
+  //   16 / 4 heads of 64   512 fresh rows 13.8 / 12.1  512 after 4096 31 / 38
+  // Two parts of q of 128 dims leave a CU no room for a second workgroup (8 x 300
+  // rows after 200 53 / 62, 512 fresh ones 30 / 24).
   const int KG = 128 / d->cache.head_dim;
   const int cols = chunk_cols(d->cache.head_dim, d->out_dtype == CBIS_F32 ? 3 : 1);
   const int want = (CBIS_PREFILL_TILE_ROWS * group + cols - 1) / cols;
+  const bool alone = KG == 1 && d->q_dtype == CBIS_F32 && d->out_dtype == CBIS_BF16;
+  const int64_t eights = (int64_t)n_tiles * d->cache.n_kv_heads * cdiv(want, 8 / KG);
+  if (blocks <= 32 && (!alone || eights <= kCUs / 2)) p.sw = 2;
   while (p.sw < 4 / KG && 4 / p.sw >= want * KG) p.sw *= 2;
   const int wh = 8 / p.sw / KG;
   p.ncg = (want + wh - 1) / wh;

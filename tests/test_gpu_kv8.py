@@ -677,3 +677,35 @@ def test_first_scores_of_minus_infinity(cbis, dev, heads, kv_heads, d, q_dtype, 
             want, mag, big = ref.attend(qv[i].reshape(heads, d), kk, vv)
             tol = ref.tolerance(want, mag, big, 101 + i, d, np.abs(c.kv[0][1]).max(), q_dtype, out_dtype)
             assert (np.abs(got[i] - want) <= tol).all(), (form, split, i)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [h for h in HEADS if h[2] > 32])
+@pytest.mark.parametrize("q_dtype,out_dtype", DTYPES)
+def test_chunk_wide_table(cbis, dev, heads, kv_heads, d, q_dtype, out_dtype):
+    """Short sequences in a table of 4096 tokens, which is what the call is laid out
+    for: its widest workgroups, and splits most of which are empty."""
+    import torch
+    c = Case(cbis, dev, kv_heads, d, 16, [450, 449], seed=heads + d + 2)
+    table = torch.full((2, 256), -5, dtype=torch.int32, device=dev)
+    table[:, :c.d_table.shape[1]] = c.d_table
+    w = heads * d
+    r = rng(7)
+    for tiles in (TILES[2], TILES[4]):
+        n = max(t[0] + t[1] for t in tiles)
+        q, qv = _as(r.standard_normal((n, w)).astype(np.float32), q_dtype, dev)
+        d_tiles = torch.tensor(tiles, dtype=torch.int32, device=dev)
+        out = torch.full((n, w), 7.0, dtype=_t(out_dtype), device=dev)
+        for split in (0, 4096):
+            a = c.desc(cbis, q, q_dtype, out, out_dtype, heads)
+            a.block_table, a.bt_stride, a.split_tokens = ptr(table), 256, split
+            need = cbis.kernels().cbis_kv8_chunk_attention_workspace_size(ctypes.byref(a), len(tiles))
+            assert (need == 0) == (split == 4096)
+            ws = _workspace(a, need, dev)
+            cbis.check(cbis.kernels().cbis_kv8_chunk_attention(ctypes.byref(a), len(tiles), ptr(d_tiles), stream()))
+            sync()
+            del ws
+            got = out.double().cpu().numpy()
+            for row, rows, seq, pos in tiles:
+                for i in {0, rows // 2, rows - 1}:
+                    c.check(got[row + i].reshape(heads, d), seq, pos + i, qv[row + i].reshape(heads, d), q_dtype,
+                            out_dtype, f"split {split}")
