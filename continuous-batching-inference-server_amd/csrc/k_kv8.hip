@@ -73,13 +73,18 @@ __device__ inline float pow2_of_byte(unsigned b) { return __uint_as_float(b << 2
 // Rows in and out of their slots.
 //
 // A workgroup of 16 waves takes up to 16 rows of 256 (fp32) or 512 (bf16) columns
-// of K and of V, a row to a wave and 16 bytes of it to a lane.  Where the rows are the 16 tokens of one
-// cache tile (a prompt's rows) the V codes are turned in LDS, so that the tile's
-// dims are written and read in whole 16-byte pieces; other rows go slot by slot.
-// With a wave to a row and no more, the 16 bytes of a V dim came from up to 8
-// XCDs, each writing its own part of the line back.  HBM-bound on large calls,
-// by latency on small ones (so the waves share nothing they need not, and the
-// code is short: it is fetched anew by every launch).
+// of K and of V, a row to a wave and 16 bytes of it to a lane.  Where the rows are
+// the 16 tokens of one cache tile (a prompt's rows) the V codes are turned in LDS,
+// so that the tile's dims are written and read in whole 16-byte pieces; other rows
+// go slot by slot.  With a wave to a row and no more, the 16 bytes of a V dim came
+// from up to 8 XCDs, each writing its own part of the line back (16355 bf16 rows of
+// 8 heads of 128 took 103 us).
+// HBM-bound on large calls: those rows are written in 23.3 us (4.3 TB/s of reads and
+// writes, a large copy's rate is 4.8), 12291 bf16 rows of 64 heads of 32 read back in
+// 25.5 (6.0).  By latency on small ones, so the waves share nothing they need not,
+// and the code is short: it is fetched anew by every launch (8 rows 2.8 us, 777
+// scattered ones read back 5.0).  Two rows to a wave of 8 give fp32 rows 5-9% and
+// cost bf16 ones 5%; four of them cost 16%.
 //
 // The rows are cut into groups where the tokens are: row r follows row r - 1 if
 // its slot is the next one of the same tile.  A window of 16 rows owns the runs
@@ -573,6 +578,13 @@ __device__ inline u32x4_t keep(bool mine, u32x4_t w) {
 // always on its way.  Page ids are read two blocks ahead, before loads that are
 // not yet wanted, since loads arrive in order and awaiting one awaits the older
 // ones; they are turned into addresses only where those are used.
+//
+// 192 rows of 256..4096, 64 heads of 32: 264 us, 6.7 TB/s (a read-only kernel reaches
+// 7.1); 16 rows of 32768: 328 and 5 of joining.  61 rows of 500..16384, 8 K/V heads
+// of 128: 185 us, 5.7 TB/s, 6.6% more than its bytes fetched: 8 heads' scale bytes
+// share a line that as many XCDs read.  (All heads of a row on one XCD gives 2.5%,
+// but leaves XCDs idle where rows are few or unsorted.)  The non-temporal loads are
+// worth 12% at 32 dims (304 us without), 3% at 128.
 template <int HD, int NH, int QP, int PP>
 __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const AttnArgs a) {
   constexpr int NK = HD / 32, ND = HD / 16;
@@ -836,21 +848,27 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
   }
 }
 
-// Chunks at head_dim 64 and 128.  A workgroup owns (tile, kv head, a group of its columns, split): column
-// c is row c / group of the tile and query head c % group of the kv head's own.
-// Each wave has 32 columns and one of KG parts of the keys (KG * HD = 128), whose
-// results are joined at the end (two heads of 64 together instead: 61 us for two
-// chunks of 512 rows after 2048 x 32 heads, two parts of the keys 45: the work
-// comes in smaller pieces).  KG blocks of 64 tokens (8 KB of K and of V) are converted to bf16 and f16 once, by all waves, into LDS
-// in the order in which the products take them; while they are multiplied the
-// next ones' codes are in registers, on their way from the cache.  The scales go in with the conversion: K's exactly, V's as 2^(byte
-// - E + 6), so that the largest code comes to 448 * 64 and what is lost of small
-// slices stays below 2^-40 of it.  The probabilities' sums are one more product,
-// with a V of ones, on the rounded values that the outputs are made of.
+// Chunks at head_dim 64 and 128.  A workgroup owns (tile, kv head, a group of its
+// columns, split): column c is row c / group of the tile and query head c % group of
+// the kv head's own.  Each wave has 32 columns and one of KG parts of the keys
+// (KG * HD = 128), whose results are joined at the end (two heads of 64 together
+// instead: 61 us for two chunks of 512 rows after 2048 x 32 heads, two parts of the
+// keys 45: the work comes in smaller pieces).  KG blocks of 64 tokens (8 KB of K and
+// of V) are converted to bf16 and f16 once, by all waves, into LDS in the order in
+// which the products take them; while they are multiplied the next ones' codes are
+// in registers, on their way from the cache.  The scales go in with the conversion:
+// K's exactly, V's as 2^(byte - E + 6), so that the largest code comes to 448 * 64
+// and what is lost of small slices stays below 2^-30 of the largest |V|.  The
+// probabilities' sums are one more product, with a V of ones, on the rounded values
+// that the outputs are made of.
 //
-// Bound by the softmax's vector instructions (per wave and block 32 fma, 32 exp2 at
-// a quarter of their rate, 16 conversions, 16 max), which overlap with the other
-// wave's products only in part.
+// 512 rows after 16384, 32 / 8 heads of 128: 143 us and 10 of joining, 0.91 PFLOP/s
+// (a large library product reaches 1.2).  MFMAs are busy 43% of the SIMDs' cycles
+// and vector instructions 52% (per wave and block 32 fma, 32 exp2 at a quarter of
+// their rate, 16 conversions, 16 max, and its share of the staging); each wave reads
+// 32 KB of operands a block from LDS, half of what that delivers meanwhile.  Two
+// groups of waves in alternate phases, one's products beside the other's softmax,
+// change nothing (176 us both; head_dim 64 218 -> 244).
 constexpr int kChunkCols = 32;  // columns of a wave at head_dim 32
 // The other head dims: 16 where three parts of q of 128 dims would not leave room
 // for the rest (28 / 4 heads of 128, 1024 fp32 rows after 2048: 32 columns spill
@@ -1246,6 +1264,11 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
 // everything: a wave has 32 columns of a kv head and every tw-th block of 64
 // tokens, straight from the cache through registers like the single rows'
 // kernel, so that waves run apart and fill each other's gaps.
+//
+// Two chunks of 512 rows after 0 and 512, 64 heads: 21.9 us, of 2048 waves with 1 to
+// 16 blocks each; 512 rows after 16384: 183.  Vector instructions are issued in
+// 65% of the SIMDs' cycles (of a block's 32 columns 32 exp2 take 512 cycles, 140
+// others 560), products in 20%.
 template <int QP, int PP>
 __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const AttnArgs a) {
   constexpr int HD = 32, ND = 2, CT = kChunkCols / 16, kPitch = HD + 4;
@@ -1480,7 +1503,9 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const At
 // The splits of a row's head joined: the mean of their outputs weighted by
 // their sums.  HD / 4 lanes hold 4 dims each; `share` such groups of a wave (a
 // power of two) take a (slot, head)'s splits in turn, a slot being a decode row
-// or a tile's row.
+// or a tile's row.  Bound by latency, so that the loads of four splits go out
+// together (64 rows after 16384 x 29 splits of 32 heads of 128, with the attention:
+// 47.5 -> 42 us); 512 rows x 4 splits of 32 heads, 34 MB, take 10 us.
 constexpr int kMergeAhead = 4;  // splits whose loads a lane has on their way
 
 template <int HD>
@@ -1663,7 +1688,7 @@ Plan plan_decode(const cbis_kv8_attn_desc* d) {
   // The waves that share a row's head block: as many as bring the waves to
   // 4096, two rounds of what the GPU holds, so that rows of half the longest
   // one's length still fill it; no more than the blocks. us by waves, MI355X:
-  //   192 rows of 256..4096 x 64 heads of 32 (3072 head blocks)  1: 285  2: 277  4: 278  8: 312
+  //   192 rows of 256..4096 x 64 heads of 32                     1: 285  2: 277  4: 278  8: 312
   //   256 rows of 100 x 64 heads of 32 (4096)                    1: 29   2: 35   4: 49   8: 84
   //   64 rows of 1000 x 64 heads of 32 (1024)                    1: 48   2: 47   4: 50   8: 62
   //   61 rows of 500..16384, 32 / 8 heads of 128 (488)           1: 563  2: 319  4: 230  8: 193

@@ -374,9 +374,11 @@ size_t cbis_kv8_attention_workspace_size(const cbis_kv8_attn_desc* d);
  * set of rows, each with its own length (the decode form).  A row with a negative
  * position attends to nothing and comes out zero; keys past
  * bt_stride * page_size are not read.  What a page's slots past the row's
- * last key hold does not matter.  Sums and statistics are fp32; with a bf16 result fp32 q is
- * used to 16 bits and the probabilities to 11, with an fp32 result q in full
- * and the probabilities to 22. */
+ * last key hold does not matter.  Sums and statistics are fp32; with a bf16
+ * result fp32 q is used to 16 bits and the probabilities to 11, with an fp32
+ * result q in full and the probabilities to 22.  V below 2^-30 of the largest
+ * |V| that the row (below: its tile) has met may count as zero.  Calls that may
+ * overlap, on two streams or as two graphs, need a workspace each. */
 int cbis_kv8_attention(const cbis_kv8_attn_desc* d, cbis_stream_t stream);
 
 /* The same for tiles of up to CBIS_PREFILL_TILE_ROWS consecutive rows of one
