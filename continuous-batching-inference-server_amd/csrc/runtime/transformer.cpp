@@ -14,6 +14,8 @@
 //    single rows and MFMA prefill attention for runs of consecutive rows of
 //    one sequence -> out-projection GEMM with bias + residual epilogue ->
 //    LayerNorm -> fc1 GEMM with bias + GELU -> fc2 GEMM with bias + residual;
+//  * over an fp8 cache the QKV GEMM leaves its rows in fp32, a launch quantises K
+//    and V into their slots, and the attention is the 8-bit calls';
 //  * steps whose shape repeats replay a captured HIP graph;
 //  * forward_step_greedy runs lm_head fused with the row argmax and top-2
 //    margin on the device (no logits stored where the GEMM reduces them).
