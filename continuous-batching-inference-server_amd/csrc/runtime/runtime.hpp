@@ -271,7 +271,7 @@ class TransformerRunner {
 
   // current step
   int M_ = 0;
-  int n_decode_ = 0, n_tiles_ = 0, n_seqs_ = 0, bt_width_ = 0, max_kv_ = 0, split_tokens_ = 0;
+  int n_decode_ = 0, n_tiles_ = 0, n_seqs_ = 0, bt_width_ = 0, max_kv_ = 0, tile_kv_ = 0, split_tokens_ = 0;
   int fused_proj_ = 0;  // this step runs attention + out-projection as one launch per layer
   size_t meta_bytes_ = 0;
   const uint8_t* stage_src_ = nullptr;  // the step's metadata in host memory (device address) ...

@@ -275,6 +275,8 @@ void TransformerRunner::prepare(int b, const int* tok, const int* pos, const int
   n_seqs_ = (int)seqs.size();
   bt_width_ = width;
   max_kv_ = (max_kv + 255) / 256 * 256;  // coarse, so steps share split shapes (and graphs)
+  // The tiles' longest, which only the 8-bit chunk attention is laid out by.
+  tile_kv_ = cfg_.kv_dtype == CBIS_FP8E4M3 && n_tiles_ ? (tiles[1] + tiles[3] + 255) / 256 * 256 : 0;
   // Steps of decode rows only, at most 64 with keys up to 768 (the attention
   // library's one-pass bound for such calls, so the fused launch reads each
   // row's keys as the separate one would): one launch per layer for the
@@ -366,7 +368,7 @@ void TransformerRunner::prepare(int b, const int* tok, const int* pos, const int
 }
 
 std::vector<int> TransformerRunner::signature() const {
-  return {M_, n_decode_, n_tiles_, n_seqs_, bt_width_, max_kv_, split_tokens_, fused_proj_};
+  return {M_, n_decode_, n_tiles_, n_seqs_, bt_width_, max_kv_, tile_kv_, split_tokens_, fused_proj_};
 }
 
 void TransformerRunner::enqueue_forward(int b, bool greedy, bool from_prev) {
@@ -479,7 +481,7 @@ void TransformerRunner::enqueue_forward(int b, bool greedy, bool from_prev) {
                  "K/V rows");
       a8.max_kv_len = max_kv_;
       cbis_check(cbis_kv8_attention(&a8, s), "attention");
-      a8.max_kv_len = 0;  // the tiles' keys are bounded by the table's width
+      a8.max_kv_len = tile_kv_;
       cbis_check(cbis_kv8_chunk_attention(&a8, n_tiles_, d_tiles_, s), "chunk attention");
       if (ln_pro) cbis_check(cbis_gemm(&g, s), "out-proj gemm");
       else cbis_check(cbis_gemm_layernorm(&g, L.ln2_w, L.ln2_b, 1e-5f, act, d_xn_, D, s), "out-proj gemm + ln2");
