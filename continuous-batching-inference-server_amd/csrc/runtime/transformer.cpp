@@ -368,7 +368,7 @@ void TransformerRunner::prepare(int b, const int* tok, const int* pos, const int
 }
 
 std::vector<int> TransformerRunner::signature() const {
-  return {M_, n_decode_, n_tiles_, n_seqs_, bt_width_, max_kv_, tile_kv_, split_tokens_, fused_proj_};
+  return {M_, n_decode_, n_tiles_, n_seqs_, bt_width_, max_kv_, split_tokens_, fused_proj_};
 }
 
 void TransformerRunner::enqueue_forward(int b, bool greedy, bool from_prev) {
@@ -551,7 +551,7 @@ void TransformerRunner::run_step(int b, bool greedy, bool from_prev) {
   // A graph names one set of step buffers (and, reading the previous step's
   // tokens, the other set's results).
   std::vector<int> sig = signature();
-  sig.insert(sig.end(), {greedy ? 1 : 0, b, from_prev ? 1 : 0});
+  sig.insert(sig.end(), {tile_kv_, greedy ? 1 : 0, b, from_prev ? 1 : 0});
   auto it = graphs_.find(sig);
   if (it == graphs_.end()) {
     if (graphs_.size() >= kMaxGraphs) {
