@@ -973,7 +973,7 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
   const int H = a.c.kv_heads, j = wave / WH;  // j: the wave's part of the keys
   const int c0 = wg0 + wave % WH * COLS;
   const bool busy = c0 < cols;  // the others stage only
-  const int first_pos = pos0 + c0 / a.group;
+  const int first_pos = min(pos0 + c0 / a.group, a.max_tok - 1);
   const int last_pos = min(pos0 + (min(c0 + COLS, cols) - 1) / a.group, a.max_tok - 1);
   int pos[CT];
   bf16v8_t q[CT][NK][QP];
@@ -1290,7 +1290,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const At
   const int c0 = cg * kChunkCols, cols = nv * a.group;
   const bool busy = in && c0 < cols;
   const int* bt = a.bt + (int64_t)td.z * a.bt_stride;
-  const int first_pos = pos0 + c0 / a.group;
+  const int first_pos = min(pos0 + c0 / a.group, a.max_tok - 1);
   const int last_pos = min(pos0 + (min(c0 + kChunkCols, cols) - 1) / a.group, a.max_tok - 1);
   int pos[CT];
   bf16v8_t q[CT][QP];

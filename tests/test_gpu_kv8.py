@@ -709,3 +709,25 @@ def test_chunk_wide_table(cbis, dev, heads, kv_heads, d, q_dtype, out_dtype):
                 for i in {0, rows // 2, rows - 1}:
                     c.check(got[row + i].reshape(heads, d), seq, pos + i, qv[row + i].reshape(heads, d), q_dtype,
                             out_dtype, f"split {split}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 8, 32), (8, 4, 64), (32, 8, 128), (28, 4, 128)])
+@pytest.mark.parametrize("first", [20, 48, 4000])
+def test_tiles_past_the_table(cbis, dev, heads, kv_heads, d, first):
+    """Whole tiles whose rows lie past the table's 48 tokens, which end inside a
+    block of 64: each sees those 48, once."""
+    import torch
+    c = Case(cbis, dev, kv_heads, d, 16, [48], seed=71)
+    w = heads * d
+    q, qv = _as(rng(72).standard_normal((70, w)).astype(np.float32), "f32", dev)
+    tiles = torch.tensor([(0, 64, 0, first), (64, 6, 0, first + 64)], dtype=torch.int32, device=dev)
+    out = torch.empty((70, w), device=dev)
+    a = c.desc(cbis, q, "f32", out, "f32", heads)
+    a.bt_stride = 3
+    ws = _workspace(a, cbis.kernels().cbis_kv8_chunk_attention_workspace_size(ctypes.byref(a), 2), dev)
+    cbis.check(cbis.kernels().cbis_kv8_chunk_attention(ctypes.byref(a), 2, ptr(tiles), stream()))
+    sync()
+    del ws
+    got = out.double().cpu().numpy().reshape(70, heads, d)
+    for i in (0, 1, 15, 16, 27, 28, 31, 32, 33, 47, 63, 64, 69):
+        c.check(got[i], 0, min(first + i, 47), qv[i].reshape(heads, d), "f32", "f32", f"row {i}")
