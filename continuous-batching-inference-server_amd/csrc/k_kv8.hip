@@ -566,11 +566,11 @@ __device__ inline u32x4_t keep(bool mine, u32x4_t w) {
   return w;
 }
 
-// Single rows.  A workgroup owns (row, NH kv heads, split); its waves take the
-// split's 64-token blocks in turn.  The 16 columns of the products are the query
-// heads: with q zero outside a kv head's own columns the scores of the NH kv
-// heads accumulate into the same four registers per product, each head in its
-// column, so one softmax serves them all; the output does the same with P.
+// What single rows and tiles of few columns share: a wave's 16 columns over the
+// 64-token blocks b0, b0 + step, .. below b1 of a row whose keys are 0 .. kv - 1, into
+// the running maximum m, the sums l, the V scales' bound E and the outputs O.
+// kCausal: the columns have last keys `pos` of their own, and every one sees the
+// keys below `full`.
 //
 // Bound by HBM while enough bytes are in flight: a block's K and V are 32
 // registers of loads each (NH * HD = 128), the next block's K is loaded as soon
@@ -578,64 +578,12 @@ __device__ inline u32x4_t keep(bool mine, u32x4_t w) {
 // always on its way.  Page ids are read two blocks ahead, before loads that are
 // not yet wanted, since loads arrive in order and awaiting one awaits the older
 // ones; they are turned into addresses only where those are used.
-//
-// 192 rows of 256..4096, 64 heads of 32: 264 us, 6.7 TB/s (a read-only kernel reaches
-// 7.1); 16 rows of 32768: 328 and 5 of joining.  61 rows of 500..16384, 8 K/V heads
-// of 128: 185 us, 5.7 TB/s, 6.6% more than its bytes fetched: 8 heads' scale bytes
-// share a line that as many XCDs read.  (All heads of a row on one XCD gives 2.5%,
-// but leaves XCDs idle where rows are few or unsorted.)  The non-temporal loads are
-// worth 12% at 32 dims (304 us without), 3% at 128.
-template <int HD, int NH, int QP, int PP>
-__global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const AttnArgs a) {
+template <int HD, int NH, int QP, int PP, bool kCausal>
+__device__ __forceinline__ void attend_keys(const AttnArgs& a, const int* bt, const bf16v8_t (&q)[HD / 32][QP], int kv, int pos,
+                                   int full, int b0, int b1, int step, int kh0, int my, int my_head, bool col_ok,
+                                   float& m, float& l, int& E, f32x4_t (&O)[HD / 16]) {
   constexpr int NK = HD / 32, ND = HD / 16;
-  constexpr int kPitch = HD + 4;
-  extern __shared__ float o_sh[];  // [wave][16][kPitch], then lse_sh [wave][16]; none where tw is 1
-  const int wave = wave_id(), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  // All rows' last splits first, their first ones at the end, where the short
-  // rows (behind the long ones, if the caller sorts them) fill the tail.  With a
-  // row's splits side by side the later (often empty) ones would fall on the
-  // same XCDs for every row: workgroup b runs on XCD b % 8.
-  // The waves are tw token parts of waves / tw head blocks.
-  const int waves = blockDim.x >> 6, hpw = waves / a.tw, groups = (a.nhb + hpw - 1) / hpw;
-  unsigned bid = blockIdx.x;
-  const int hb = (int)(bid % (unsigned)groups) * hpw + wave / a.tw, tpart = wave % a.tw;
-  bid /= (unsigned)groups;
-  const int ri = (int)(bid % (unsigned)a.n_rows), split = a.nsplit - 1 - (int)(bid / (unsigned)a.n_rows);
-  const int row = a.rows ? a.rows[ri] : ri;
-  const int kv = min(a.row_pos[row], a.max_tok - 1) + 1;  // keys 0 .. kv - 1, none when <= 0
-  const int* bt = a.bt + (a.row_bt ? a.row_bt[row] : row) * a.bt_stride;
-  // Columns: column n is query head h0 + n, of kv head kh0 + n / group (of kh0
-  // where a kv head has 16 or more).
-  int kh0, h0, ncol;
-  if (NH == 1 && a.group > 16) {
-    const int sub = (a.group + 15) / 16;
-    kh0 = hb / sub;
-    h0 = kh0 * a.group + hb % sub * 16;
-    ncol = min(16, (kh0 + 1) * a.group - h0);
-  } else {
-    kh0 = hb * NH;
-    h0 = kh0 * a.group;
-    ncol = min(NH, a.c.kv_heads - kh0) * a.group;
-  }
-  if (hb >= a.nhb) ncol = 0;
-  const bool col_ok = n < ncol;
-  const int my = !col_ok ? -1 : NH == 1 ? 0 : n / a.group;
-  const int my_head = min(kh0 + max(my, 0), a.c.kv_heads - 1);
-
-  bf16v8_t q[NK][QP];
-#pragma unroll
-  for (int s = 0; s < NK; ++s)
-    load_q8<QP>(a, (int64_t)row * a.ldq + (int64_t)(h0 + n) * HD + q_dim<HD>(s, g), col_ok, 1.f, q[s]);
-
-  float m = kLowest, l = 0.f;
-  int E = 0;
-  f32x4_t O[ND];
-#pragma unroll
-  for (int i = 0; i < ND; ++i) O[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  const int nblk = kv > 0 ? (kv + kBlk - 1) / kBlk : 0;
-  const int b0 = split * a.split_blocks + tpart, step = a.tw;
-  const int b1 = ncol <= 0 ? 0 : split == a.nsplit - 1 ? nblk : min(nblk, (split + 1) * a.split_blocks);
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int tlast = (kv - 1) >> 4;
   const int64_t codes = (int64_t)a.c.kv_heads * HD * kTile;
   // Lane offsets inside a tile; kv heads past the last one read the last.
@@ -700,14 +648,15 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
       load_k_block(tile_offset(a.c, kpage, k_tile(b + step)));
       __builtin_amdgcn_sched_barrier(0);
       const int valid = min(max(kv - (b * kBlk + g * kTile), 0), kTile);  // tokens of tile g inside the row
-      const bool tail = (b + 1) * kBlk > kv;
+      const bool tail = (b + 1) * kBlk > kv, mask = kCausal ? (b + 1) * kBlk > full : tail;
+      const int seen = kCausal ? pos + 1 - (b * kBlk + g * kTile) : valid;  // of them, by the column
       float top = -INFINITY;
 #pragma unroll
       for (int p = 0; p < 4; ++p)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float x = S[p][i] * (pow2_of_byte(byte_of(kb[p], i)) * a.qscale);
-          if (tail && 4 * p + i >= valid) x = -INFINITY;
+          if (mask && 4 * p + i >= seen) x = -INFINITY;
           S[p][i] = x;
           top = fmaxf(top, x);
         }
@@ -727,7 +676,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if ((int)byte_of(vb[d], i) == kBadByte) {
-              if (col_ok) l = NAN;
+              if (col_ok && 4 * d + i < seen) l = NAN;
               vb[d] &= ~(0xFFu << (8 * i));
             }
             bmax = max(bmax, (int)byte_of(vb[d], i));
@@ -796,6 +745,72 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
       __builtin_amdgcn_sched_barrier(0);
     }
   }
+}
+
+// Single rows.  A workgroup owns (row, NH kv heads, split); its waves take the
+// split's 64-token blocks in turn.  The 16 columns of the products are the query
+// heads: with q zero outside a kv head's own columns the scores of the NH kv
+// heads accumulate into the same four registers per product, each head in its
+// column, so one softmax serves them all; the output does the same with P.
+//
+// 192 rows of 256..4096, 64 heads of 32: 264 us, 6.7 TB/s (a read-only kernel reaches
+// 7.1); 16 rows of 32768: 328 and 5 of joining.  61 rows of 500..16384, 8 K/V heads
+// of 128: 185 us, 5.7 TB/s, 6.6% more than its bytes fetched: 8 heads' scale bytes
+// share a line that as many XCDs read.  (All heads of a row on one XCD gives 2.5%,
+// but leaves XCDs idle where rows are few or unsorted.)  The non-temporal loads are
+// worth 12% at 32 dims (304 us without), 3% at 128.
+template <int HD, int NH, int QP, int PP>
+__global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const AttnArgs a) {
+  constexpr int NK = HD / 32, ND = HD / 16;
+  constexpr int kPitch = HD + 4;
+  extern __shared__ float o_sh[];  // [wave][16][kPitch], then lse_sh [wave][16]; none where tw is 1
+  const int wave = wave_id(), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  // All rows' last splits first, their first ones at the end, where the short
+  // rows (behind the long ones, if the caller sorts them) fill the tail.  With a
+  // row's splits side by side the later (often empty) ones would fall on the
+  // same XCDs for every row: workgroup b runs on XCD b % 8.
+  // The waves are tw token parts of waves / tw head blocks.
+  const int waves = blockDim.x >> 6, hpw = waves / a.tw, groups = (a.nhb + hpw - 1) / hpw;
+  unsigned bid = blockIdx.x;
+  const int hb = (int)(bid % (unsigned)groups) * hpw + wave / a.tw, tpart = wave % a.tw;
+  bid /= (unsigned)groups;
+  const int ri = (int)(bid % (unsigned)a.n_rows), split = a.nsplit - 1 - (int)(bid / (unsigned)a.n_rows);
+  const int row = a.rows ? a.rows[ri] : ri;
+  const int kv = min(a.row_pos[row], a.max_tok - 1) + 1;  // keys 0 .. kv - 1, none when <= 0
+  const int* bt = a.bt + (a.row_bt ? a.row_bt[row] : row) * a.bt_stride;
+  // Columns: column n is query head h0 + n, of kv head kh0 + n / group (of kh0
+  // where a kv head has 16 or more).
+  int kh0, h0, ncol;
+  if (NH == 1 && a.group > 16) {
+    const int sub = (a.group + 15) / 16;
+    kh0 = hb / sub;
+    h0 = kh0 * a.group + hb % sub * 16;
+    ncol = min(16, (kh0 + 1) * a.group - h0);
+  } else {
+    kh0 = hb * NH;
+    h0 = kh0 * a.group;
+    ncol = min(NH, a.c.kv_heads - kh0) * a.group;
+  }
+  if (hb >= a.nhb) ncol = 0;
+  const bool col_ok = n < ncol;
+  const int my = !col_ok ? -1 : NH == 1 ? 0 : n / a.group;
+  const int my_head = min(kh0 + max(my, 0), a.c.kv_heads - 1);
+
+  bf16v8_t q[NK][QP];
+#pragma unroll
+  for (int s = 0; s < NK; ++s)
+    load_q8<QP>(a, (int64_t)row * a.ldq + (int64_t)(h0 + n) * HD + q_dim<HD>(s, g), col_ok, 1.f, q[s]);
+
+  float m = kLowest, l = 0.f;
+  int E = 0;
+  f32x4_t O[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) O[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  const int nblk = kv > 0 ? (kv + kBlk - 1) / kBlk : 0;
+  const int b0 = split * a.split_blocks + tpart;
+  const int b1 = ncol <= 0 ? 0 : split == a.nsplit - 1 ? nblk : min(nblk, (split + 1) * a.split_blocks);
+  attend_keys<HD, NH, QP, PP, false>(a, bt, q, kv, kv - 1, kv, b0, b1, a.tw, kh0, my, my_head, col_ok, m, l, E, O);
 
   // Each wave's normalised output and log2 sum, then, where several waves share
   // the columns, their weighted mean.
@@ -944,8 +959,72 @@ struct ChunkStage {
 template <int HD>
 constexpr size_t chunk_lds(int waves) {
   const size_t stages = 2 * sizeof(ChunkStage<HD>) + waves * 64 * sizeof(_Float16);
-  const size_t join = HD == 128 ? 0 : (size_t)waves * 32 * (HD + 5) * sizeof(float);
+  const size_t join = (size_t)waves * (HD == 128 ? 16 : 32) * (HD + 5) * sizeof(float);  // 128: of few columns
   return stages > join ? stages : join;
+}
+
+// A tile of few columns (the last rows of a prompt, a short turn after a long one):
+// its W waves are parts of the keys, 16 columns each, straight from the cache like the
+// single rows.  In the other way the waves past the columns would only convert for the
+// rest.  us, that way / this one:
+//   16 heads of 128, 8 rows after 16384     40 / 25    32 heads of 64  32 / 22
+//   32 / 8 heads of 128, 4 rows after 4096  17 / 15, 8 after 1000  14.4 / 13.1, and of
+//     more than 32 columns, 14 rows after 16384  29 / 36: each wave converts for 16
+//     columns only
+constexpr int kFewCols = 32;
+
+template <int HD, int W, int QP, int PP, typename Finish>
+__device__ __forceinline__ void few_columns(const AttnArgs& a, const int* bt, float* o_sh, int kh, int split, int cols,
+                                            int row0, int pos0, Finish finish) {
+  constexpr int NK = HD / 32, ND = HD / 16, kPitch = HD + 4;
+  const int wave = wave_id(), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  int cw = 1;  // waves that the columns take
+  while (16 * cw < cols) cw *= 2;
+  const int parts = W / cw, part = wave / cw, c0 = wave % cw * 16, c = c0 + n;
+  const bool col_ok = c < cols;
+  const int t = c / a.group, pos = col_ok ? min(pos0 + t, a.max_tok - 1) : -1;
+  bf16v8_t q[NK][QP];
+#pragma unroll
+  for (int s = 0; s < NK; ++s)
+    load_q8<QP>(a, (int64_t)(row0 + t) * a.ldq + (int64_t)(kh * a.group + c % a.group) * HD + q_dim<HD>(s, g), col_ok, 1.f, q[s]);
+  const int kv = c0 < cols ? min(pos0 + (min(c0 + 16, cols) - 1) / a.group, a.max_tok - 1) + 1 : 0;
+  const int nblk = kv > 0 ? (kv + kBlk - 1) / kBlk : 0;
+  const int b0 = split * a.split_blocks + part;
+  const int b1 = split == a.nsplit - 1 ? nblk : min(nblk, (split + 1) * a.split_blocks);
+  float m = kLowest, l = 0.f;
+  int E = 0;
+  f32x4_t O[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) O[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  attend_keys<HD, 1, QP, PP, true>(a, bt, q, kv, pos, min(pos0 + c0 / a.group, a.max_tok - 1) + 1, b0, b1, parts, kh, 0,
+                                   kh, col_ok, m, l, E, O);
+
+  l = column_sum(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float* lse_sh = o_sh + W * 16 * kPitch;
+  if (g == 0) lse_sh[wave * 16 + n] = l == 0.f ? -INFINITY : m - 8.f + __log2f(l);
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+    *(float4*)(o_sh + (wave * 16 + n) * kPitch + 16 * i + 4 * g) =
+        make_float4(ldexpf(O[i][0] * inv, E - 127), ldexpf(O[i][1] * inv, E - 127), ldexpf(O[i][2] * inv, E - 127),
+                    ldexpf(O[i][3] * inv, E - 127));
+  __syncthreads();
+  for (int i = threadIdx.x; i < cols * (HD / 4); i += W * 64) {
+    const int col = i / (HD / 4), d = i % (HD / 4) * 4;
+    float top = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int x = 0; x < parts; ++x) top = fmaxf(top, lse_sh[x * cw * 16 + col]);
+    for (int x = 0; x < parts; ++x) {
+      const float lw = lse_sh[x * cw * 16 + col];
+      if (lw == -INFINITY) continue;
+      const float f = fast_exp2(lw - top);
+      const float4 y = *(const float4*)(o_sh + (x * cw * 16 + col) * kPitch + d);
+      sum += f;
+      o[0] += f * y.x; o[1] += f * y.y; o[2] += f * y.z; o[3] += f * y.w;
+    }
+    const float norm = sum == 0.f ? 0.f : 1.f / sum;
+    for (int e = 0; e < 4; ++e) o[e] *= norm;
+    finish(col, d, o, sum == 0.f ? -INFINITY : top + __log2f(sum));
+  }
 }
 
 template <int HD, int SW, int QP, int PP>
@@ -970,6 +1049,21 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
   const int cols = nv * a.group, wg0 = cg * WH * COLS;
   if (wg0 >= cols) return;
   const int* bt = a.bt + (int64_t)btr * a.bt_stride;
+  // A column's result: normalised outputs and the log2 of its sum.
+  auto finish = [&](int c, int d, const float* o, float lse) {
+    const int t = c / a.group, head = kh * a.group + c % a.group;
+    if (a.nsplit == 1) {
+      store_out4(a, (int64_t)(row0 + t) * a.ldo + (int64_t)head * HD + d, o);
+    } else {
+      const int64_t at = ((tile * CBIS_PREFILL_TILE_ROWS + t) * a.nsplit + split) * a.n_heads + head;
+      *(float4*)(a.part + at * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+      if (d == 0) a.lse[at] = lse;
+    }
+  };
+  if (cols <= (W < 4 || COLS < 32 ? 16 : kFewCols)) {
+    few_columns<HD, W, QP, PP>(a, bt, (float*)lds, kh, split, cols, row0, pos0, finish);
+    return;
+  }
   const int H = a.c.kv_heads, j = wave / WH;  // j: the wave's part of the keys
   const int c0 = wg0 + wave % WH * COLS;
   const bool busy = c0 < cols;  // the others stage only
@@ -1204,17 +1298,6 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
       lds_barrier();
     }
   }
-  // A column's result: normalised outputs and the log2 of its sum.
-  auto finish = [&](int c, int d, const float* o, float lse) {
-    const int t = c / a.group, head = kh * a.group + c % a.group;
-    if (a.nsplit == 1) {
-      store_out4(a, (int64_t)(row0 + t) * a.ldo + (int64_t)head * HD + d, o);
-    } else {
-      const int64_t at = ((tile * CBIS_PREFILL_TILE_ROWS + t) * a.nsplit + split) * a.n_heads + head;
-      *(float4*)(a.part + at * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
-      if (d == 0) a.lse[at] = lse;
-    }
-  };
   constexpr int kPitch = HD + 4, WC = WH * COLS;
   float* o_sh = (float*)lds;                 // [part][column][kPitch]
   float* lse_sh = o_sh + KG * WC * kPitch;   // [part][column]
@@ -1771,6 +1854,9 @@ Plan plan_chunk(const cbis_kv8_attn_desc* d, int n_tiles) {
     per = KG;
     while (4 * per * per < blocks) per += KG;
     per = std::max<int64_t>({per, 2, cdiv(blocks, std::max<int64_t>(1, kCUs / units))});
+    // A CU holds two of the smaller workgroups: where keys are long, splits for both
+    // (32 heads of 64: 512 rows after 16384 185 -> 146, 3 x 28 after 12149 75 -> 62).
+    if (p.sw > 1 && per > 48) per = std::max<int64_t>(48, cdiv(blocks, std::max<int64_t>(1, 2 * kCUs / units)));
   }
   set_splits(d, blocks, per, &p);
   return p;

@@ -115,8 +115,9 @@ TransformerRunner::TransformerRunner(const ModelWeights& weights, PagedKVCache& 
   hip_check(hipHostGetDevicePointer((void**)&hd_logits_, h_logits_, 0), "hipHostGetDevicePointer logits");
   // Split-KV partials: the automatic split keeps rows * splits <= 2048 + rows.
   ws_bytes_ = (2048 + R) * (size_t)cfg_.n_heads * (cfg_.head_dim + 4) * 4;
-  // The 8-bit calls' own splits keep rows * splits * heads <= 16384.
-  if (kv8) ws_bytes_ = (size_t)16384 * (cfg_.head_dim + 1) * 4;
+  // The 8-bit calls' own splits keep rows * splits * heads <= 32768 (without grouped
+  // heads; a tile counts as 64 rows).
+  if (kv8) ws_bytes_ = (size_t)32768 * (cfg_.head_dim + 1) * 4;
   hip_check(hipMalloc(&d_ws_, ws_bytes_), "hipMalloc attention workspace");
   // Split-K workspace: the largest any of the step's GEMM shapes asks for at
   // any row count up to max_total_rows (through cbis_gemm_layernorm, whose

@@ -138,3 +138,22 @@ def test_host_cache_of_fp8_pages(cbis):
     for ps, hd in ((8, 32), (24, 32), (16, 48), (16, 16), (16, 256)):
         with pytest.raises(cbis.CbisError, match="fp8 K/V pages"):
             cbis.PagedKVCache(2, 8, ps, 3, hd, "fp8", alloc_device=False)
+
+
+@pytest.mark.parametrize("heads", [1, 2, 5, 8, 16, 32, 40, 64])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_workspace_bound_without_groups(cbis, heads, d):
+    """What a runner sets aside once covers every step's calls: rows (64 to a tile)
+    x splits x heads is at most 32768."""
+    a = cbis.Kv8AttnDesc()
+    a.cache.n_kv_heads, a.cache.head_dim, a.cache.page_size, a.cache.num_pages = heads, d, 16, 1
+    a.n_heads, a.bt_stride, a.q_dtype = heads, 1 << 16, cbis.F32
+    k = cbis.kernels()
+    for out in (cbis.F32, cbis.BF16):
+        a.out_dtype = out
+        for kv in (1, 500, 1000, 2049, 5000, 10000, 20000, 32768, 100000, 1 << 20):
+            a.max_kv_len = kv
+            for n in (1, 2, 3, 4, 5, 7, 8, 12, 16, 24, 33, 64, 100, 200, 1000):
+                a.n_rows = n
+                assert k.cbis_kv8_attention_workspace_size(ctypes.byref(a)) <= 32768 * (d + 1) * 4
+                assert k.cbis_kv8_chunk_attention_workspace_size(ctypes.byref(a), n) <= 32768 * (d + 1) * 4

@@ -731,3 +731,41 @@ def test_tiles_past_the_table(cbis, dev, heads, kv_heads, d, first):
     got = out.double().cpu().numpy().reshape(70, heads, d)
     for i in (0, 1, 15, 16, 27, 28, 31, 32, 33, 47, 63, 64, 69):
         c.check(got[i], 0, min(first + i, 47), qv[i].reshape(heads, d), "f32", "f32", f"row {i}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 8, 64), (16, 4, 64), (40, 8, 64), (4, 4, 128), (32, 8, 128), (28, 4, 128),
+                                              (17, 1, 128), (24, 1, 64)])
+@pytest.mark.parametrize("q_dtype,out_dtype", DTYPES)
+def test_tiles_of_few_rows(cbis, dev, heads, kv_heads, d, q_dtype, out_dtype):
+    """A few rows after many keys, whose waves share the keys: whole and in splits, laid
+    out for long keys and for short ones; rows before position 0; a K and a V slice of
+    NaN that only the later rows see."""
+    import torch
+    c = Case(cbis, dev, kv_heads, d, 16, [1300], seed=heads + d + 3)
+    for which, token, head in ((0, 1293, kv_heads - 1), (1, 1292, 0)):
+        pool = c.pools[which].cpu().numpy()
+        code, byte = ref.slot_index(kv_heads, d, 16, which == 1, c.table[0, token // 16], token % 16)
+        pool[code[head]], pool[byte[head]] = 0, 255
+        c.pools[which].copy_(torch.from_numpy(pool))
+        c.kv[0][which][token, head] = np.nan
+    w = heads * d
+    q, qv = _as(rng(82).standard_normal((20, w)).astype(np.float32), q_dtype, dev, 8)
+    tiles = [(0, 4, 0, 1290), (4, 1, 0, 70), (5, 8, 0, -3), (13, 2, 0, 1023), (15, 1, 0, 0), (16, 1, 0, 1299)]
+    d_tiles = torch.tensor(tiles, dtype=torch.int32, device=dev)
+    for split, max_kv in ((0, 1300), (0, 40000), (64, 1300), (512, 1300)):
+        table = torch.full((1, 2560), -5, dtype=torch.int32, device=dev)
+        table[:, :c.d_table.shape[1]] = c.d_table
+        out = torch.full((20, w + 8), 7.0, dtype=_t(out_dtype), device=dev)
+        a = c.desc(cbis, q, q_dtype, out, out_dtype, heads)
+        a.block_table, a.bt_stride, a.max_kv_len, a.split_tokens = ptr(table), 2560, max_kv, split
+        need = cbis.kernels().cbis_kv8_chunk_attention_workspace_size(ctypes.byref(a), len(tiles))
+        ws = _workspace(a, need, dev)
+        cbis.check(cbis.kernels().cbis_kv8_chunk_attention(ctypes.byref(a), len(tiles), ptr(d_tiles), stream()))
+        sync()
+        del ws
+        got = out.double().cpu().numpy()
+        assert (got[17:] == 7.0).all() and (got[:, w:] == 7.0).all()
+        for row, rows, seq, pos in tiles:
+            for i in range(rows):
+                c.check(got[row + i, :w].reshape(heads, d), seq, pos + i, qv[row + i].reshape(heads, d), q_dtype, out_dtype,
+                        f"split {split} max {max_kv} row {row + i}")
