@@ -1814,13 +1814,17 @@ Plan plan_chunk(const cbis_kv8_attn_desc* d, int n_tiles) {
     //   512 rows after 16384                     1: 224   2048: 192   4096: 201   8192: 220
     //   512 fresh rows                           1: 12.5  2048: 10.8  4096: 13.8  8192: 21.6
     //   16 rows after 32000                      1: 118   2048: 61    4096: 61    8192: 61
-    while (p.tw < kDecodeWaves && units * p.tw < 2048 && p.tw < part) p.tw *= 2;
+    // But 8 only where that is no more than a workgroup per CU, which does not hold
+    // two (of four it holds three): 3 x 64 rows after 1000 18.6 with 8, 14.7 with 4, 3 x
+    // 20 after 5000 40 and 31.
+    while (p.tw < (units <= kCUs ? 8 : 4) && units * p.tw < 2048 && p.tw < part) p.tw *= 2;
     p.waves = std::max(p.tw, 4);
-    // Splits for one workgroup of eight per CU, from 48 blocks on.  us by tokens of
+    // Splits for what the CUs hold at once, from 48 blocks on.  us by tokens of
     // a split (* the rule's): 64 rows of 64 heads after 2000  1024: 19  2048*: 14,
     // after 4000  1024: 22  2048*: 18  4096: 20, after 32000  8192: 64  16384*: 60
     // 32768: 93; 64 rows of 8 heads after 4000  256*: 11.4  1024: 14  4096: 19.
-    if (blocks >= 48) set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, kCUs / units)), 4), &p);
+    const int64_t room = units <= kCUs ? kCUs : 3 * kCUs;
+    if (blocks >= 48) set_splits(d, blocks, std::max<int64_t>(cdiv(blocks, std::max<int64_t>(1, room / units)), 4), &p);
     else set_splits(d, blocks, blocks, &p);
     return p;
   }
