@@ -676,7 +676,7 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, const int* bt, co
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if ((int)byte_of(vb[d], i) == kBadByte) {
-              if (col_ok && 4 * d + i < seen) l = NAN;
+              if (col_ok && (!kCausal || 4 * d + i < seen)) l = NAN;
               vb[d] &= ~(0xFFu << (8 * i));
             }
             bmax = max(bmax, (int)byte_of(vb[d], i));
