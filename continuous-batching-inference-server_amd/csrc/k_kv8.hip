@@ -879,8 +879,8 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_decode_kernel(const Att
 //
 // 512 rows after 16384, 32 / 8 heads of 128: 143 us and 10 of joining, 0.91 PFLOP/s
 // (a large library product reaches 1.2).  MFMAs are busy 43% of the SIMDs' cycles
-// and vector instructions 52% (per wave and block 32 fma, 32 exp2 at a quarter of
-// their rate, 16 conversions, 16 max, and its share of the staging); each wave reads
+// and vector instructions 52% (per wave and block 300: the products' 68, 32 fma, 32
+// exp2 at half the rate, 16 conversions, 16 max, and its share of the staging); each wave reads
 // 32 KB of operands a block from LDS, half of what that delivers meanwhile.  Two
 // groups of waves in alternate phases, one's products beside the other's softmax,
 // change nothing (176 us both; head_dim 64 218 -> 244).
@@ -1350,8 +1350,8 @@ __global__ __launch_bounds__(512 / SW) void kv8_chunk_kernel(const AttnArgs a) {
 //
 // Two chunks of 512 rows after 0 and 512, 64 heads: 21.9 us, of 2048 waves with 1 to
 // 16 blocks each; 512 rows after 16384: 183.  Vector instructions are issued in
-// 65% of the SIMDs' cycles (of a block's 32 columns 32 exp2 take 512 cycles, 140
-// others 560), products in 20%.
+// 63% of the SIMDs' cycles (some 310 for a block's 32 columns, 32 of them exp2 at
+// half the rate, by the counters), products in 20%.
 template <int QP, int PP>
 __global__ __launch_bounds__(kDecodeWaves * 64) void kv8_chunk32_kernel(const AttnArgs a) {
   constexpr int HD = 32, ND = 2, CT = kChunkCols / 16, kPitch = HD + 4;
