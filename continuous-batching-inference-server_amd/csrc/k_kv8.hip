@@ -83,8 +83,11 @@ __device__ inline float pow2_of_byte(unsigned b) { return __uint_as_float(b << 2
 // writes, a large copy's rate is 4.8), 12291 bf16 rows of 64 heads of 32 read back in
 // 25.5 (6.0).  By latency on small ones, so the waves share nothing they need not,
 // and the code is short: it is fetched anew by every launch (8 rows 2.8 us, 777
-// scattered ones read back 5.0).  Two rows to a wave of 8 give fp32 rows 5-9% and
-// cost bf16 ones 5%; four of them cost 16%.
+// scattered ones read back 5.0).  Two whole rows to a wave of 8 give fp32 rows 5-9%
+// and cost bf16 ones 5%; four of them cost 16%.
+// Rows of at most half or a quarter of a wave's columns go two or four to a wave
+// (34812 rows of 256 bf16 columns written 20.7 -> 15.6 us, read back 16.2 -> 11.4; of
+// 128 columns 18.7 -> 9.7 and 15 -> 9.9).
 //
 // The rows are cut into groups where the tokens are: row r follows row r - 1 if
 // its slot is the next one of the same tile.  A window of 16 rows owns the runs
@@ -227,10 +230,12 @@ __device__ inline void values(const uint32_t* w, float scale, float* x) {
   }
 }
 
-// What a workgroup of the row kernels works on.
-template <int HD, int N>
+// What a workgroup of the row kernels works on.  R rows to a wave (1, 2 or 4, where
+// they are as narrow as that), 64 / R lanes each.
+template <int HD, int N, int R>
 struct RowPlace {
   int wave, lane, part, col, head, dim, at, end;
+  int row;  // the lane's row of the group
   int64_t window, codes;
   bool col_ok;
   RowSlots rs;
@@ -239,7 +244,8 @@ struct RowPlace {
     lane = threadIdx.x & 63;
     window = (int64_t)(blockIdx.x / a.parts) * kTile;
     part = (int)(blockIdx.x % a.parts);
-    col = (part * 64 + lane) * N;
+    col = (part * 64 + lane % (64 / R)) * N;
+    row = wave * R + lane / (64 / R);
     col_ok = col < a.c.kv_heads * HD;
     head = col / HD;
     dim = col % HD;
@@ -252,36 +258,48 @@ struct RowPlace {
   __device__ bool whole(int stop) const {
     return stop - at == kTile && ((rs.starts >> (at + 1)) & 0x7FFF) == 0 && (rs.live >> at & 1);
   }
-  __device__ bool mine(int stop) const { return at + wave < stop && (rs.live >> (at + wave) & 1); }
+  __device__ bool mine(int stop) const {
+    const int i = at + (R == 1 ? wave : row);
+    return i < stop && (rs.live >> i & 1);
+  }
   // Offset of the tile that row at + i lies in, and its slot there.
   __device__ int64_t tile(const RowsArgs& a, int i, int* slot) const {
     const int page = __builtin_amdgcn_readlane(rs.page, at + i), off = __builtin_amdgcn_readlane(rs.off, at + i);
+    return tile_at(a, page, off, slot);
+  }
+  // Those of the lane's own row (by all lanes of the wave).
+  __device__ int64_t my_tile(const RowsArgs& a, int* slot) const {
+    if constexpr (R == 1) return tile(a, wave, slot);
+    else return tile_at(a, __shfl(rs.page, at + row, 64), __shfl(rs.off, at + row, 64), slot);
+  }
+  __device__ static int64_t tile_at(const RowsArgs& a, int page, int off, int* slot) {
     *slot = off & (kTile - 1);
     return (((int64_t)page << a.c.tshift) + (off >> 4)) * a.c.tile_bytes;
   }
 };
 
-template <typename T, int HD>
-__global__ __launch_bounds__(kRowThreads) void kv8_scatter_kernel(const RowsArgs a) {
+template <typename T, int HD, int R>
+__global__ __launch_bounds__(kRowThreads / R) void kv8_scatter_kernel(const RowsArgs a) {
   constexpr int N = kLaneCols<T>, NW = N / 4;
-  __shared__ uint32_t turn[kTile][64 * NW];  // V codes of the group's rows, 4 columns to a dword
-  RowPlace<HD, N> r(a);
+  __shared__ uint32_t turn[kTile][64 / R * NW];  // V codes of the group's rows, 4 columns to a dword
+  RowPlace<HD, N, R> r(a);
   for (int stop; r.at < r.end; r.at = stop) {
     stop = group_end(r.rs.starts, r.at, r.end);
     const bool whole = r.whole(stop);
-    if (r.mine(stop)) {
-      const int64_t row = r.window + r.at + r.wave;
+    const bool mine = r.mine(stop);
+    if (R == 1 ? mine : __ballot(mine) != 0) {
+      const int64_t row = r.window + r.at + (R == 1 ? r.wave : r.row);
       float xk[N] = {}, xv[N] = {};
-      if (r.col_ok) {
+      if (mine && r.col_ok) {
         load_row((const T*)a.k + row * a.ldk + r.col, xk);
         load_row((const T*)a.v + row * a.ldv + r.col, xv);
       }
       int slot, bk, bv;
-      const int64_t tile = r.tile(a, r.wave, &slot);
+      const int64_t tile = r.my_tile(a, &slot);
       uint32_t wk[NW], wv[NW];
       quantise<HD, N>(xk, wk, &bk);
       quantise<HD, N>(xv, wv, &bv);
-      if (r.col_ok) {
+      if (mine && r.col_ok) {
         uint8_t* dk = a.c.k + tile + ((int64_t)r.head * kTile + slot) * HD + r.dim;
         if constexpr (NW == 1) *(uint32_t*)dk = wk[0];
         else *(u32x2_t*)dk = u32x2_t{wk[0], wk[1]};
@@ -291,7 +309,7 @@ __global__ __launch_bounds__(kRowThreads) void kv8_scatter_kernel(const RowsArgs
         }
         if (whole) {
 #pragma unroll
-          for (int i = 0; i < NW; ++i) turn[r.wave][r.lane * NW + i] = wv[i];
+          for (int i = 0; i < NW; ++i) turn[R == 1 ? r.wave : r.row][r.lane % (64 / R) * NW + i] = wv[i];
         } else {
           uint8_t* dv = a.c.v + tile + (int64_t)r.col * kTile + slot;
 #pragma unroll
@@ -320,11 +338,11 @@ __global__ __launch_bounds__(kRowThreads) void kv8_scatter_kernel(const RowsArgs
 }
 
 // Read back: the same groups the other way.
-template <typename T, int HD>
-__global__ __launch_bounds__(kRowThreads) void kv8_gather_kernel(const RowsArgs a) {
+template <typename T, int HD, int R>
+__global__ __launch_bounds__(kRowThreads / R) void kv8_gather_kernel(const RowsArgs a) {
   constexpr int N = kLaneCols<T>, NW = N / 4;
-  __shared__ uint32_t turn[kTile][64 * NW];
-  RowPlace<HD, N> r(a);
+  __shared__ uint32_t turn[kTile][64 / R * NW];
+  RowPlace<HD, N, R> r(a);
   for (int stop; r.at < r.end; r.at = stop) {
     stop = group_end(r.rs.starts, r.at, r.end);
     const bool whole = r.whole(stop);
@@ -347,16 +365,18 @@ __global__ __launch_bounds__(kRowThreads) void kv8_gather_kernel(const RowsArgs 
       }
       __syncthreads();
     }
+    int slot;
+    int64_t tile;
+    if constexpr (R > 1) tile = r.my_tile(a, &slot);
     if (r.mine(stop) && r.col_ok) {
-      int slot;
-      const int64_t tile = r.tile(a, r.wave, &slot);
+      if constexpr (R == 1) tile = r.my_tile(a, &slot);
       const uint32_t* src = (const uint32_t*)(a.c.k + tile + ((int64_t)r.head * kTile + slot) * HD + r.dim);
       uint32_t wk[NW], wv[NW];
 #pragma unroll
       for (int i = 0; i < NW; ++i) wk[i] = src[i];
       if (whole) {
 #pragma unroll
-        for (int i = 0; i < NW; ++i) wv[i] = turn[r.wave][r.lane * NW + i];
+        for (int i = 0; i < NW; ++i) wv[i] = turn[R == 1 ? r.wave : r.row][r.lane % (64 / R) * NW + i];
       } else {
         const uint8_t* sv = a.c.v + tile + (int64_t)r.col * kTile + slot;
 #pragma unroll
@@ -366,7 +386,7 @@ __global__ __launch_bounds__(kRowThreads) void kv8_gather_kernel(const RowsArgs 
       }
       const float sk = pow2_of_byte(a.c.k[tile + r.codes + r.head * kTile + slot]);
       const float sv = pow2_of_byte(a.c.v[tile + r.codes + r.head * kTile + slot]);
-      const int64_t row = r.window + r.at + r.wave;
+      const int64_t row = r.window + r.at + (R == 1 ? r.wave : r.row);
       float x[N];
       values<N>(wk, sk, x);
       store_row((T*)a.k + row * a.ldk + r.col, x);
@@ -1677,17 +1697,25 @@ int make_pages(const cbis_kv8_cache* c, Pages* p, const char* who) {
   return CBIS_OK;
 }
 
+template <typename T, int HD>
+void rows_launch(bool gather, int rows, const RowsArgs& a, unsigned grid, hipStream_t s) {
+  const int threads = kRowThreads / rows;
+  if constexpr (HD <= 16 * kLaneCols<T>) {
+    if (rows == 4 && gather) return kv8_gather_kernel<T, HD, 4><<<grid, threads, 0, s>>>(a);
+    if (rows == 4) return kv8_scatter_kernel<T, HD, 4><<<grid, threads, 0, s>>>(a);
+  }
+  if (rows == 2 && gather) kv8_gather_kernel<T, HD, 2><<<grid, threads, 0, s>>>(a);
+  else if (rows == 2) kv8_scatter_kernel<T, HD, 2><<<grid, threads, 0, s>>>(a);
+  else if (gather) kv8_gather_kernel<T, HD, 1><<<grid, threads, 0, s>>>(a);
+  else kv8_scatter_kernel<T, HD, 1><<<grid, threads, 0, s>>>(a);
+}
+
 template <typename T>
 void rows_launch(bool gather, const RowsArgs& a, unsigned grid, hipStream_t s) {
-  if (gather) {
-    if (a.c.head_dim == 32) kv8_gather_kernel<T, 32><<<grid, kRowThreads, 0, s>>>(a);
-    else if (a.c.head_dim == 64) kv8_gather_kernel<T, 64><<<grid, kRowThreads, 0, s>>>(a);
-    else kv8_gather_kernel<T, 128><<<grid, kRowThreads, 0, s>>>(a);
-  } else {
-    if (a.c.head_dim == 32) kv8_scatter_kernel<T, 32><<<grid, kRowThreads, 0, s>>>(a);
-    else if (a.c.head_dim == 64) kv8_scatter_kernel<T, 64><<<grid, kRowThreads, 0, s>>>(a);
-    else kv8_scatter_kernel<T, 128><<<grid, kRowThreads, 0, s>>>(a);
-  }
+  const int width = a.c.kv_heads * a.c.head_dim, rows = width <= 16 * kLaneCols<T> ? 4 : width <= 32 * kLaneCols<T> ? 2 : 1;
+  if (a.c.head_dim == 32) rows_launch<T, 32>(gather, rows, a, grid, s);
+  else if (a.c.head_dim == 64) rows_launch<T, 64>(gather, rows, a, grid, s);
+  else rows_launch<T, 128>(gather, rows, a, grid, s);
 }
 
 int kv8_rows(bool gather, const cbis_kv8_cache* c, int n_rows, int dtype, const void* K, int64_t ldk, const void* V,

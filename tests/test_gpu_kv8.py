@@ -769,3 +769,12 @@ def test_tiles_of_few_rows(cbis, dev, heads, kv_heads, d, q_dtype, out_dtype):
             for i in range(rows):
                 c.check(got[row + i, :w].reshape(heads, d), seq, pos + i, qv[row + i].reshape(heads, d), q_dtype, out_dtype,
                         f"split {split} max {max_kv} row {row + i}")
+
+
+@pytest.mark.parametrize("kv_heads,d,page_size,n,pad", [
+    (1, 32, 16, 70, 0), (2, 32, 32, 150, 3), (3, 32, 16, 77, 0), (8, 32, 16, 170, 1), (1, 64, 16, 90, 1),
+    (2, 64, 16, 48, 0), (4, 64, 32, 200, 2), (1, 128, 64, 130, 0), (2, 128, 16, 65, 4)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_narrow_rows(cbis, dev, kv_heads, d, page_size, n, pad, dtype):
+    """Rows of which a wave takes several, or just does not."""
+    test_scatter_then_gather(cbis, dev, kv_heads, d, page_size, n, pad, dtype)
